@@ -222,7 +222,7 @@ def _run_own(s, case):
     if case['op'] == 'policy':
         r = losses.policy_loss(s['logp'], s['adv'], s['old'], s['ref'], clip=CLIP, clip_high=CLIP_HIGH,
                                dual_clip=case['dual'] or None, kl_coef=KL_COEF, kl=case['kl'], reduction=case['reduction'],
-                               **s['which'])
+                               per_token=case['adv'] == 'token', **s['which'])
         return r.loss, r.grad, r.policy, r.kl, r.clip_fraction, r.ratio
     if case['op'] == 'pairs':
         r = losses.preference_loss(s['logp'], s['ref'], beta=BETA, kind=case['kind'], label_smoothing=SMOOTH,
