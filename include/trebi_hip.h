@@ -339,6 +339,117 @@ int trebi_trainer_set_bucket_event(trebi_trainer* tr, void* event);
 int trebi_trainer_step(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps,
                        int ema_mode, float ema_decay, void* stream);
 
+/* ---- fine-tuning ------------------------------------------------------------------
+ * What follows the imitation of the training step above: policy-gradient and preference fine-tuning of the denoiser,
+ * and the clipping that keeps such steps stable.  No counterpart in the reference.  These calls allocate nothing, keep
+ * no state and only enqueue (graph-capturable); tables and workspaces are the caller's, one per call in flight.  Sums
+ * are taken in float64 and in a fixed order: results do not change from run to run. */
+typedef enum { TREBI_F32 = 0, TREBI_BF16 = 1, TREBI_F16 = 2 } trebi_dtype;
+
+/* Global gradient norm over many tensors (each contiguous, aligned to its type; numels may be 0), and clipping:
+ *   n = s * (sum g^2)^(1/2) | s * sum |g| | s * max |g|   (norm_type 0 | 1 | 2),   s = grad_scale (1 / loss scale)
+ *   c = s * min(1, max_norm / (n + 1e-6));                 every gradient becomes c * g, rounded once to its type
+ * A norm that is NaN makes every gradient NaN; an infinite one makes the finite ones 0 (torch.nn.utils.clip_grad_norm_).
+ * trebi_grad_set_fill is host code: it cuts the tensors into chunks and fills a HOST table of trebi_grad_set_bytes()
+ * bytes, which the caller copies to the device (256-byte aligned) and keeps, with `out`, while the tensors stay where
+ * they are.  trebi_grad_clip scales in place, or with `out` leaves the gradients alone and writes the scaled values back
+ * to back (in the tensors' order) as `total` float32.  norm_out: dev [1], nullable in trebi_grad_clip. */
+typedef struct { int n_tensors, n_chunks; int64_t total; } trebi_grad_set;
+size_t trebi_grad_set_bytes(int n_tensors, const int64_t* numels);
+int trebi_grad_set_fill(int n_tensors, const void* const* tensors, const int64_t* numels, const int* dtypes, void* host_table,
+                        size_t table_bytes, trebi_grad_set* out);
+size_t trebi_grad_workspace_bytes(const trebi_grad_set* set);
+int trebi_grad_norm(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float grad_scale,
+                    float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+int trebi_grad_clip(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float max_norm,
+                    float grad_scale, float* out /* nullable: in place */, float* norm_out, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Which tokens count.  Padded: [rows, len], of which the first lengths[r] of a row (null: all) where mask is not 0
+ * (null: everywhere).  Packed: `len` tokens, row r is [cu_seqlens[r], cu_seqlens[r+1]), cu_seqlens not decreasing; tokens
+ * before the first and behind the last row belong to none.  Offsets and lengths outside the tensor are cut to it.  What
+ * a token that does not count holds (NaN too) reaches no output; its gradient is 0. */
+typedef struct {
+  int64_t rows, len;
+  int packed;
+  const int32_t* lengths;      /* dev [rows] or null */
+  const int32_t* cu_seqlens;   /* dev [rows + 1] */
+  const uint8_t* mask;         /* dev or null */
+  int64_t mask_row_stride, mask_col_stride;
+} trebi_token_desc;
+
+/* Clipped policy loss with a KL term, and its gradient, in one pass over the tokens:
+ *   d = logp - old (old null: 0),  rho = e^d,  delta = ref - logp
+ *   pg = -A rho, held at the border without gradient beyond it: A > 0 and rho > 1 + clip_high; A < 0 and rho < 1 - clip_low;
+ *        with dual_clip also A < 0 and rho > dual_clip
+ *   kl = -delta | delta^2 / 2 | e^delta - delta - 1   (kl_kind 1 | 2 | 3; ref null: 0)
+ *   loss = sum_i w_i (pg_i + kl_coef kl_i);  w = 1 / tokens (reduction 0), 1 / (rows that are not empty * tokens of the row)
+ *          (1), 1 / denominator (2)
+ *   grad = grad_scale * d loss / d logp, contiguous, in logp's type (rounded once); null: the loss alone
+ * Strides in elements; packed tensors have column stride 1.  advantages: float32, column stride 0 = one a row.
+ * stats: dev [5] loss, sum w pg, sum w kl, share of tokens beyond a border, mean rho.  Nothing valid: all 0. */
+typedef struct {
+  int dtype;                   /* of logp, logp_old, logp_ref and grad */
+  const void *logp, *logp_old, *logp_ref;
+  int64_t logp_row_stride, logp_col_stride, old_row_stride, old_col_stride, ref_row_stride, ref_col_stride;
+  const float* advantages;
+  int64_t adv_row_stride, adv_col_stride;
+  void* grad;
+  float* stats;
+  float clip_low, clip_high, dual_clip /* 0: off */, kl_coef;
+  int kl_kind, reduction;
+  double denominator;
+  float grad_scale;
+} trebi_policy_loss_desc;
+size_t trebi_policy_loss_workspace_bytes(const trebi_token_desc* tokens);
+int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const trebi_policy_loss_desc* desc, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Preference loss over pairs of rows (row k < rows/2 is preferred to row k + rows/2), and its gradient:
+ *   D_r = sum over the row's valid tokens of logp - ref (ref null: logp), with `average` divided by their number
+ *   h = D_chosen - D_rejected,  z = beta h - margin
+ *   l = (1 - e) softplus(-z) + e softplus(z) | max(0, 1 - z) | (z / beta - 1 / (2 beta))^2   (kind 0 | 1 | 2; e: smoothing)
+ *   loss = sum weights l / denominator (0: the number of pairs); a pair with an empty row gives nothing
+ * grad: like the policy loss.  chosen_reward / rejected_reward: dev [rows/2], beta D.  stats: dev [3] loss, share of the
+ * pairs that count with h > 0, their mean z. */
+typedef struct {
+  int dtype;
+  const void *logp, *logp_ref;
+  int64_t logp_row_stride, logp_col_stride, ref_row_stride, ref_col_stride;
+  const float* weights;        /* dev [rows/2] or null: 1 */
+  void* grad;
+  float *chosen_reward, *rejected_reward, *stats;
+  float beta, label_smoothing, margin;
+  int kind, average;
+  double denominator;
+  float grad_scale;
+} trebi_preference_loss_desc;
+size_t trebi_preference_loss_workspace_bytes(const trebi_token_desc* tokens);
+int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const trebi_preference_loss_desc* desc, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Log-probability of the reverse step x_t -> x_prev that trebi_ddpm_update draws (diffusion.py:153-185), given the net's
+ * output `pred` on x_t, and grad_pred = grad_logp[b] * d logp[b] / d pred:
+ *   x0 = pred, or sqrt_recip[t] x_t - sqrt_recipm1[t] pred with those tables (a net that predicts the noise),
+ *   clamped to [-1, 1] with clip_denoised;  mu = coef1[t] x0 + coef2[t] x_t
+ *   logp = sum over elements of -(x_prev - mu)^2 / (2 e^plv) - (log 2 pi + plv) / 2
+ * without the elements that a condition overwrites (observation part of the rows cond_index); 0 at t = 0, where the step
+ * adds no noise.  pred, x, x_prev: [B, horizon, transition_dim], contiguous inside a candidate, candidate strides in
+ * elements; grad_pred contiguous.  Tables: DEVICE [n_timesteps].  t as everywhere in this library. */
+typedef struct {
+  int horizon, transition_dim, action_dim, observation_dim, n_timesteps;
+  int clip_denoised;
+  int n_cond, cond_index[4];
+  int64_t pred_stride, x_stride, x_prev_stride;
+  const float *posterior_log_variance, *coef1, *coef2;
+  const float *sqrt_recip_alphas_cumprod, *sqrt_recipm1_alphas_cumprod;   /* both null: the net predicts x0 */
+} trebi_transition_desc;
+int trebi_transition_logp(trebi_ctx* ctx, const trebi_transition_desc* desc, const float* pred, const float* x,
+                          const float* x_prev, const int64_t* t, int64_t B, float* logp, void* stream);
+int trebi_transition_logp_grad(trebi_ctx* ctx, const trebi_transition_desc* desc, const float* pred, const float* x,
+                               const float* x_prev, const int64_t* t, const float* grad_logp, int64_t B, float* grad_pred,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,374 @@
+// finetune.inl -- host side of the fine-tuning operators (included at the end of trebi.hip): argument checks and launch
+// shapes of the gradient norm (gradnorm.hip), the policy and preference losses and the transition log-probability
+// (losses.hip).  Nothing here allocates, synchronises or keeps state: tables and workspaces are the caller's.
+#include "finetune.h"
+
+namespace {
+
+// The context's device for the length of a call; the caller's current device is put back.
+struct DeviceGuard {
+  int before = -1;
+  hipError_t err;
+  explicit DeviceGuard(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device) err = hipSetDevice(device);
+    else if (err == hipSuccess) before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+#define ON_DEVICE(ctx)                    \
+  DeviceGuard on_device((ctx)->device);   \
+  HIPCHK(on_device.err)
+
+// Elements of a chunk: about four chunks for each of the workgroups, so that ends of tensors even out, and never
+// less than a workgroup reads at one go four times over.
+long long grad_chunk(long long total) {
+  const long long per = (total + 4 * GRAD_BLOCKS - 1) / (4 * GRAD_BLOCKS);
+  return std::min<long long>(std::max<long long>((per + 4095) / 4096 * 4096, 4096), 1 << 28);
+}
+size_t grad_tensors_bytes(int n) { return ((size_t)n * sizeof(GradTensor) + 255) / 256 * 256; }
+
+int grad_totals(int n, const int64_t* numels, long long* total, long long* chunks) {
+  if (n < 1 || !numels) return fail(TREBI_BAD_ARG, "at least one tensor is needed");
+  *total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (numels[i] < 0) return fail(TREBI_BAD_ARG, "tensor %d has a negative size", i);
+    *total += numels[i];
+  }
+  const long long c = grad_chunk(*total);
+  *chunks = 0;
+  for (int i = 0; i < n; ++i) *chunks += (numels[i] + c - 1) / c;
+  if (*chunks > 0x7fffffff) return fail(TREBI_UNSUPPORTED_CONFIG, "too many tensors for one set");
+  return 0;
+}
+
+int grad_args(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float grad_scale, void* ws,
+              size_t ws_bytes, GradP* p) {
+  if (!ctx || !set || !table || !ws) return fail(TREBI_BAD_ARG, "null argument");
+  if (norm_type < 0 || norm_type > 2) return fail(TREBI_BAD_ARG, "norm_type must be 0 (two-norm), 1 (one-norm) or 2 (largest)");
+  if (set->n_tensors < 1 || set->n_chunks < 0) return fail(TREBI_BAD_ARG, "the set was not filled");
+  if (!(grad_scale >= 0.f)) return fail(TREBI_BAD_ARG, "grad_scale must not be negative");
+  if (ws_bytes < trebi_grad_workspace_bytes(set))
+    return fail(TREBI_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", ws_bytes, trebi_grad_workspace_bytes(set));
+  p->tensors = (const GradTensor*)table;
+  p->chunks = (const GradChunk*)((const char*)table + grad_tensors_bytes(set->n_tensors));
+  p->n_chunks = set->n_chunks;
+  p->norm_type = norm_type;
+  p->grad_scale = grad_scale;
+  p->part = (double*)ws;
+  p->n_part = std::max(1, std::min(set->n_chunks, GRAD_BLOCKS));
+  return 0;
+}
+
+size_t al256(size_t n) { return (n + 255) / 256 * 256; }
+
+int token_args(const trebi_token_desc& d, TokenP* t) {
+  if (d.rows < 0 || d.len < 0 || d.rows > (1ll << 40) || d.len > (1ll << 40)) return fail(TREBI_BAD_SHAPE, "bad number of rows or tokens");
+  if (d.packed) {
+    if (!d.cu_seqlens) return fail(TREBI_BAD_ARG, "packed tokens need cu_seqlens");
+    if (d.rows < 1) return fail(TREBI_BAD_SHAPE, "packed tokens need at least one sequence");
+    if (d.lengths) return fail(TREBI_BAD_ARG, "lengths belong to padded rows");
+    if (d.len > 0x7fffffff) return fail(TREBI_UNSUPPORTED_CONFIG, "cu_seqlens is 32-bit: at most 2^31 - 1 packed tokens");
+    if (d.mask && d.mask_col_stride != 1) return fail(TREBI_BAD_ARG, "a packed mask is contiguous");
+  } else {
+    if (d.cu_seqlens) return fail(TREBI_BAD_ARG, "cu_seqlens belongs to packed tokens");
+    if (d.len > 0 && d.rows > (1ll << 46) / d.len) return fail(TREBI_BAD_SHAPE, "too many tokens");
+  }
+  t->rows = d.rows;
+  t->len = d.len;
+  t->n = d.packed ? d.len : d.rows * d.len;
+  t->packed = d.packed ? 1 : 0;
+  t->lengths = d.lengths;
+  t->cu = d.cu_seqlens;
+  t->mask = d.mask;
+  t->mrs = d.mask_row_stride;
+  t->mcs = d.mask_col_stride;
+  return 0;
+}
+
+// policy workspace: partial counts, partial sums, a count for each row
+size_t policy_bytes(const trebi_token_desc& d) {
+  return al256(COUNT_BLOCKS * sizeof(NormPart)) + al256(LOSS_PARTS * LOSS_VALS * sizeof(double)) +
+         (d.mask ? al256((size_t)d.rows * sizeof(int)) : 0);
+}
+
+constexpr int PAIR_BLOCKS = LOSS_PARTS;
+// Rows are split over workgroups where whole pairs would leave the card idle: fewer pairs than 2 a CU, and rows of
+// more than one turn of a workgroup.  (Lengths on the device do not matter for the choice, nor for the result.)
+int pair_splits(const trebi_token_desc& d) {
+  const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len;
+  if (d.rows / 2 >= 512 || len <= 4096) return 0;
+  return (int)std::max<long long>(1, std::min<long long>(LOSS_PARTS / d.rows, (len + 4095) / 4096));
+}
+size_t pair_bytes(const trebi_token_desc& d) {
+  const int s = pair_splits(d);
+  return al256(PAIR_BLOCKS * 4 * sizeof(double)) + (s ? al256((size_t)d.rows * s * 2 * sizeof(double)) : 0);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------------------------------------------
+// global gradient norm
+// ---------------------------------------------------------------------------------------------------------------
+extern "C" size_t trebi_grad_set_bytes(int n_tensors, const int64_t* numels) {
+  long long total, chunks;
+  if (grad_totals(n_tensors, numels, &total, &chunks)) return 0;
+  return grad_tensors_bytes(n_tensors) + al256((size_t)std::max<long long>(chunks, 1) * sizeof(GradChunk));
+}
+
+extern "C" int trebi_grad_set_fill(int n_tensors, const void* const* tensors, const int64_t* numels, const int* dtypes,
+                                   void* host_table, size_t table_bytes, trebi_grad_set* out) {
+  long long total, chunks;
+  if (!tensors || !dtypes || !host_table || !out) return fail(TREBI_BAD_ARG, "null argument");
+  if (int e = grad_totals(n_tensors, numels, &total, &chunks)) return e;
+  if (table_bytes < trebi_grad_set_bytes(n_tensors, numels)) return fail(TREBI_WORKSPACE_TOO_SMALL, "table of %zu bytes", table_bytes);
+  // a byte of two tensors would be scaled twice, by two workgroups at once
+  try {
+    std::vector<std::pair<uintptr_t, uintptr_t>> span;
+    for (int i = 0; i < n_tensors; ++i)
+      if (numels[i] > 0) span.push_back({(uintptr_t)tensors[i], (uintptr_t)tensors[i] + (size_t)numels[i] * (dtypes[i] == TREBI_F32 ? 4 : 2)});
+    std::sort(span.begin(), span.end());
+    for (size_t i = 1; i < span.size(); ++i)
+      if (span[i].first < span[i - 1].second) return fail(TREBI_BAD_ARG, "two of the tensors overlap (or one is given twice)");
+  } catch (const std::exception& e) {
+    return fail(TREBI_HIP_ERROR, "out of host memory: %s", e.what());
+  }
+  const long long c = grad_chunk(total);
+  GradTensor* t = (GradTensor*)host_table;
+  GradChunk* ch = (GradChunk*)((char*)host_table + grad_tensors_bytes(n_tensors));
+  long long at = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    if (dtypes[i] < 0 || dtypes[i] > 2) return fail(TREBI_BAD_ARG, "tensor %d has an unknown type %d", i, dtypes[i]);
+    const size_t size = dtypes[i] == TREBI_F32 ? 4 : 2;
+    if (numels[i] && (!tensors[i] || (uintptr_t)tensors[i] % size)) return fail(TREBI_BAD_ARG, "tensor %d is null or not aligned to its type", i);
+    t[i] = GradTensor{(void*)tensors[i], (long long)numels[i], at, dtypes[i], 0};
+    at += numels[i];
+    for (long long o = 0; o < numels[i]; o += c) *ch++ = GradChunk{o, i, (int)std::min<long long>(c, numels[i] - o)};
+  }
+  out->n_tensors = n_tensors;
+  out->n_chunks = (int)chunks;
+  out->total = total;
+  return 0;
+}
+
+extern "C" size_t trebi_grad_workspace_bytes(const trebi_grad_set* set) { return set ? GRAD_BLOCKS * sizeof(double) : 0; }
+
+extern "C" int trebi_grad_norm(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float grad_scale,
+                               float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
+  GradP p{};
+  if (int e = grad_args(ctx, set, table, norm_type, grad_scale, workspace, workspace_bytes, &p)) return e;
+  if (!norm_out) return fail(TREBI_BAD_ARG, "norm_out is null");
+  p.norm_out = norm_out;
+  ON_DEVICE(ctx);
+  HIPCHK(launch_grad_partials(p, (hipStream_t)stream));
+  HIPCHK(launch_grad_finish(p, nullptr, (hipStream_t)stream));
+  return 0;
+}
+
+extern "C" int trebi_grad_clip(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float max_norm,
+                               float grad_scale, float* out, float* norm_out, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  GradP p{};
+  if (int e = grad_args(ctx, set, table, norm_type, grad_scale, workspace, workspace_bytes, &p)) return e;
+  if (!(max_norm >= 0.f)) return fail(TREBI_BAD_ARG, "max_norm must not be negative");
+  p.max_norm = max_norm;
+  p.out = out;
+  p.norm_out = norm_out;
+  ON_DEVICE(ctx);
+  HIPCHK(launch_grad_partials(p, (hipStream_t)stream));
+  HIPCHK(launch_grad_scale(p, (hipStream_t)stream));
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// clipped policy loss
+// ---------------------------------------------------------------------------------------------------------------
+extern "C" size_t trebi_policy_loss_workspace_bytes(const trebi_token_desc* d) { return d ? policy_bytes(*d) : 0; }
+
+extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const trebi_policy_loss_desc* d, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  if (!ctx || !tokens || !d || !workspace) return fail(TREBI_BAD_ARG, "null argument");
+  PolicyP p{};
+  if (int e = token_args(*tokens, &p.tk)) return e;
+  const bool empty = p.tk.n == 0;
+  if (!d->stats || (!empty && (!d->logp || !d->advantages))) return fail(TREBI_BAD_ARG, "null argument");
+  if (d->dtype < 0 || d->dtype > 2) return fail(TREBI_BAD_ARG, "unknown type %d", d->dtype);
+  if (d->kl_kind < 1 || d->kl_kind > 3) return fail(TREBI_BAD_ARG, "kl_kind must be 1, 2 or 3");
+  if (d->reduction < 0 || d->reduction > 2) return fail(TREBI_BAD_ARG, "reduction must be 0 (token), 1 (sequence) or 2 (denominator)");
+  if (!(d->clip_low >= 0.f) || !(d->clip_high >= 0.f)) return fail(TREBI_BAD_ARG, "clip ranges must not be negative");
+  if (d->dual_clip != 0.f && !(d->dual_clip > 1.f)) return fail(TREBI_BAD_ARG, "dual_clip must be above 1 (or 0: off)");
+  if (d->reduction == 2 && !(d->denominator > 0.0)) return fail(TREBI_BAD_ARG, "denominator must be positive");
+  if (workspace_bytes < policy_bytes(*tokens)) return fail(TREBI_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, policy_bytes(*tokens));
+  p.lp = d->logp; p.old = d->logp_old; p.ref = d->logp_ref;
+  p.lrs = d->logp_row_stride; p.lcs = d->logp_col_stride;
+  p.ors = d->old_row_stride; p.ocs = d->old_col_stride;
+  p.rrs = d->ref_row_stride; p.rcs = d->ref_col_stride;
+  p.adv = d->advantages; p.ars = d->adv_row_stride; p.acs = d->adv_col_stride;
+  p.grad = d->grad;
+  // the borders in the log, in float64, of the float32 ranges that the caller gave; the ratio held there is 1 + range
+  p.hi = std::log1p((double)d->clip_high);
+  p.lo = d->clip_low < 1.f ? std::log1p(-(double)d->clip_low) : -INFINITY;
+  p.dual = d->dual_clip > 1.f ? std::log((double)d->dual_clip) : INFINITY;
+  p.vhi = (float)(1.0 + (double)d->clip_high);
+  p.vlo = (float)(1.0 - (double)d->clip_low);
+  p.vdual = d->dual_clip;
+  p.kl_coef = d->kl_coef; p.kl = d->kl_kind; p.mode = d->reduction; p.gscale = d->grad_scale;
+  p.stats = d->stats;
+  TokenP& t = p.tk;
+  const long long L = t.len;
+  if (!t.packed && t.rows == 1) {                                     // strides that no step uses
+    p.lrs = p.ors = p.rrs = t.mrs = L;
+    if (p.acs) p.ars = L;
+  }
+  if (!t.packed && L == 1) {
+    p.lcs = p.ocs = p.rcs = t.mcs = 1;
+    p.acs = 0;
+  }
+  const bool flat_lp = t.packed ? p.lcs == 1 : p.lcs == 1 && p.lrs == L;
+  const bool flat_old = !p.old || (t.packed ? p.ocs == 1 : p.ocs == 1 && p.ors == L);
+  const bool flat_ref = !p.ref || (t.packed ? p.rcs == 1 : p.rcs == 1 && p.rrs == L);
+  const bool flat_adv = p.acs == 0 || (t.packed ? p.acs == 1 : p.acs == 1 && p.ars == L);
+  const bool flat_mask = !t.mask || (t.packed ? t.mcs == 1 : t.mcs == 1 && t.mrs == L);
+  p.flat = flat_lp && flat_old && flat_ref && flat_adv && flat_mask;
+  if (t.packed && !p.flat) return fail(TREBI_UNSUPPORTED_CONFIG, "packed tensors are contiguous");
+  const bool all = !t.packed && !t.lengths && !t.mask;
+  if (p.mode == 2) p.fixed = 1.0 / d->denominator;
+  else if (all && !empty) p.fixed = 1.0 / (double)(p.mode == 0 ? t.n : t.rows);
+  char* w = (char*)workspace;
+  p.np = (NormPart*)w; w += al256(COUNT_BLOCKS * sizeof(NormPart));
+  p.part = (double*)w; w += al256(LOSS_PARTS * LOSS_VALS * sizeof(double));
+  p.counts = t.mask && p.mode == 1 ? (int*)w : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  ON_DEVICE(ctx);
+  if (!empty && (p.fixed == 0.0 || p.counts)) {
+    p.nnp = (int)std::min<long long>(COUNT_BLOCKS, std::max<long long>(1, t.mask ? t.rows : (t.rows + 255) / 256));
+    HIPCHK(launch_token_counts(p, st));
+  }
+  int blocks = 0;
+  if (!empty) {
+    const long long turns = (t.n + 2047) / 2048;                       // 256 threads x 8 tokens
+    const long long per = (turns + LOSS_PARTS - 1) / LOSS_PARTS;
+    p.per = per * 2048;
+    blocks = (int)((turns + per - 1) / per);
+    HIPCHK(launch_policy(p, d->dtype, blocks, st));
+  }
+  HIPCHK(launch_policy_finish(p, blocks, st));
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// preference loss
+// ---------------------------------------------------------------------------------------------------------------
+extern "C" size_t trebi_preference_loss_workspace_bytes(const trebi_token_desc* d) { return d && d->rows > 0 ? pair_bytes(*d) : 256; }
+
+extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const trebi_preference_loss_desc* d,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  if (!ctx || !tokens || !d || !workspace) return fail(TREBI_BAD_ARG, "null argument");
+  PairP p{};
+  if (int e = token_args(*tokens, &p.tk)) return e;
+  if (p.tk.rows < 2 || p.tk.rows % 2) return fail(TREBI_BAD_SHAPE, "%lld rows: chosen and rejected rows come in pairs", (long long)p.tk.rows);
+  if (!d->stats || !d->chosen_reward || !d->rejected_reward || (p.tk.n > 0 && !d->logp)) return fail(TREBI_BAD_ARG, "null argument");
+  if (d->dtype < 0 || d->dtype > 2) return fail(TREBI_BAD_ARG, "unknown type %d", d->dtype);
+  if (d->kind < 0 || d->kind > 2) return fail(TREBI_BAD_ARG, "kind must be 0 (sigmoid), 1 (hinge) or 2 (ipo)");
+  if (!(d->beta > 0.f)) return fail(TREBI_BAD_ARG, "beta must be positive");
+  if (!(d->label_smoothing >= 0.f) || !(d->label_smoothing < 0.5f)) return fail(TREBI_BAD_ARG, "label_smoothing must lie in [0, 0.5)");
+  if (d->denominator < 0.0 || d->denominator != d->denominator) return fail(TREBI_BAD_ARG, "denominator must be positive (0: the number of pairs)");
+  if (workspace_bytes < pair_bytes(*tokens)) return fail(TREBI_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, pair_bytes(*tokens));
+  p.pairs = p.tk.rows / 2;
+  p.lp = d->logp; p.ref = d->logp_ref;
+  p.lrs = d->logp_row_stride; p.lcs = d->logp_col_stride;
+  p.rrs = d->ref_row_stride; p.rcs = d->ref_col_stride;
+  if (p.tk.packed && (p.lcs != 1 || (p.ref && p.rcs != 1))) return fail(TREBI_UNSUPPORTED_CONFIG, "packed tensors are contiguous");
+  p.weights = d->weights;
+  p.grad = p.tk.n > 0 ? d->grad : nullptr;
+  p.beta = d->beta; p.margin = d->margin; p.smooth = d->label_smoothing; p.gscale = d->grad_scale;
+  p.inv_p = 1.0 / (d->denominator > 0.0 ? d->denominator : (double)p.pairs);
+  p.kind = d->kind; p.average = d->average ? 1 : 0;
+  p.rew_c = d->chosen_reward; p.rew_r = d->rejected_reward;
+  p.stats = d->stats;
+  p.part = (double*)workspace;
+  p.rowpart = (double*)((char*)workspace + al256(PAIR_BLOCKS * 4 * sizeof(double)));
+  p.splits = pair_splits(*tokens);
+  hipStream_t st = (hipStream_t)stream;
+  ON_DEVICE(ctx);
+  if (p.splits) {
+    p.nparts = (int)p.pairs;
+    HIPCHK(launch_pairs_split(p, d->dtype, st));
+  } else {
+    const long long len = p.tk.packed ? (p.tk.n + p.tk.rows - 1) / p.tk.rows : p.tk.len;
+    p.group = len <= 128 ? 16 : len <= 1024 ? 64 : 256;
+    const long long per = 256 / p.group;
+    const int blocks = (int)std::min<long long>(PAIR_BLOCKS, (p.pairs + per - 1) / per);
+    p.nparts = blocks;
+    HIPCHK(launch_pairs_whole(p, d->dtype, blocks, st));
+  }
+  HIPCHK(launch_pairs_finish(p, st));
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// transition log-probability
+// ---------------------------------------------------------------------------------------------------------------
+static int transition_args(trebi_ctx* ctx, const trebi_transition_desc* d, const float* pred, const float* x, const float* x_prev,
+                           const int64_t* t, int64_t B, TransP* p) {
+  if (!ctx || !d) return fail(TREBI_BAD_ARG, "null argument");
+  if (B < 0) return fail(TREBI_BAD_SHAPE, "negative batch");
+  if (d->horizon < 1 || d->transition_dim < 1 || d->action_dim < 0 || d->observation_dim < 0 || d->n_timesteps < 1 ||
+      d->action_dim + d->observation_dim > d->transition_dim || (long long)d->horizon * d->transition_dim > 1 << 28)
+    return fail(TREBI_BAD_SHAPE, "inconsistent dimensions");
+  if (B > 0 && (!pred || !x || !x_prev || !t)) return fail(TREBI_BAD_ARG, "null argument");
+  if (!d->posterior_log_variance || !d->coef1 || !d->coef2) return fail(TREBI_BAD_ARG, "null schedule table");
+  if ((d->sqrt_recip_alphas_cumprod == nullptr) != (d->sqrt_recipm1_alphas_cumprod == nullptr))
+    return fail(TREBI_BAD_ARG, "sqrt_recip_alphas_cumprod and sqrt_recipm1_alphas_cumprod go together");
+  if (d->n_cond < 0 || d->n_cond > 4) return fail(TREBI_UNSUPPORTED_CONFIG, "at most 4 conditioned timesteps are supported");
+  const int H = d->horizon, D = d->transition_dim;
+  p->B = B; p->H = H; p->D = D; p->T = d->n_timesteps;
+  p->pred = pred; p->x = x; p->xp = x_prev;
+  p->prs = d->pred_stride; p->xrs = d->x_stride; p->xprs = d->x_prev_stride;
+  p->t = (const long long*)t;
+  p->plv = d->posterior_log_variance; p->c1 = d->coef1; p->c2 = d->coef2;
+  p->ra = d->sqrt_recip_alphas_cumprod; p->rm = d->sqrt_recipm1_alphas_cumprod;
+  p->clamp = d->clip_denoised ? 1 : 0;
+  long long free_elems = (long long)H * D;
+  for (int k = 0; k < d->n_cond; ++k) {
+    const int h = d->cond_index[k];
+    if (h < 0 || h >= H) return fail(TREBI_BAD_SHAPE, "conditioned index %d outside the horizon", h);
+    bool again = false;                                   // the same index twice covers its elements once
+    for (int j = 0; j < k; ++j) again = again || d->cond_index[j] == h;
+    if (again) continue;
+    p->skip_lo[p->n_skip] = h * D + d->action_dim;
+    p->skip_hi[p->n_skip] = h * D + d->action_dim + d->observation_dim;
+    ++p->n_skip;
+    free_elems -= d->observation_dim;
+  }
+  p->half_const = 0.5 * (double)free_elems;
+  return 0;
+}
+
+extern "C" int trebi_transition_logp(trebi_ctx* ctx, const trebi_transition_desc* d, const float* pred, const float* x,
+                                     const float* x_prev, const int64_t* t, int64_t B, float* logp, void* stream) {
+  TransP p{};
+  if (int e = transition_args(ctx, d, pred, x, x_prev, t, B, &p)) return e;
+  if (B == 0) return 0;
+  if (!logp) return fail(TREBI_BAD_ARG, "logp is null");
+  p.logp = logp;
+  ON_DEVICE(ctx);
+  HIPCHK(launch_transition(p, 0, (hipStream_t)stream));
+  return 0;
+}
+
+extern "C" int trebi_transition_logp_grad(trebi_ctx* ctx, const trebi_transition_desc* d, const float* pred, const float* x,
+                                          const float* x_prev, const int64_t* t, const float* grad_logp, int64_t B, float* grad_pred,
+                                          void* stream) {
+  TransP p{};
+  if (int e = transition_args(ctx, d, pred, x, x_prev, t, B, &p)) return e;
+  if (B == 0) return 0;
+  if (!grad_logp || !grad_pred) return fail(TREBI_BAD_ARG, "null argument");
+  p.g = grad_logp;
+  p.dpred = grad_pred;
+  ON_DEVICE(ctx);
+  HIPCHK(launch_transition(p, 1, (hipStream_t)stream));
+  return 0;
+}

@@ -2453,3 +2453,8 @@ extern "C" double trebi_net_flops(const trebi_net* net, int backward) {
 extern "C" int trebi_debug_read_wstamps(unsigned long long* out);
 #endif
 #include "trainer.inl"
+
+// ------------------------------------------------------------------------------------
+// fine-tuning operators: host side
+// ------------------------------------------------------------------------------------
+#include "finetune.inl"

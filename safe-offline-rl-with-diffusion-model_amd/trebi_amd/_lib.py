@@ -50,6 +50,43 @@ class LayerInfo(C.Structure):
                 ('pro_xhat', TensorRef), ('pro_gain', TensorRef), ('pro_stats', TensorRef)]
 
 
+class GradSet(C.Structure):
+    _fields_ = [('n_tensors', C.c_int), ('n_chunks', C.c_int), ('total', C.c_int64)]
+
+
+class TokenDesc(C.Structure):
+    _fields_ = [('rows', C.c_int64), ('len', C.c_int64), ('packed', C.c_int), ('lengths', C.c_void_p),
+                ('cu_seqlens', C.c_void_p), ('mask', C.c_void_p), ('mask_row_stride', C.c_int64),
+                ('mask_col_stride', C.c_int64)]
+
+
+class PolicyLossDesc(C.Structure):
+    _fields_ = [('dtype', C.c_int), ('logp', C.c_void_p), ('logp_old', C.c_void_p), ('logp_ref', C.c_void_p),
+                ('logp_row_stride', C.c_int64), ('logp_col_stride', C.c_int64), ('old_row_stride', C.c_int64),
+                ('old_col_stride', C.c_int64), ('ref_row_stride', C.c_int64), ('ref_col_stride', C.c_int64),
+                ('advantages', C.c_void_p), ('adv_row_stride', C.c_int64), ('adv_col_stride', C.c_int64),
+                ('grad', C.c_void_p), ('stats', C.c_void_p), ('clip_low', C.c_float), ('clip_high', C.c_float),
+                ('dual_clip', C.c_float), ('kl_coef', C.c_float), ('kl_kind', C.c_int), ('reduction', C.c_int),
+                ('denominator', C.c_double), ('grad_scale', C.c_float)]
+
+
+class PreferenceLossDesc(C.Structure):
+    _fields_ = [('dtype', C.c_int), ('logp', C.c_void_p), ('logp_ref', C.c_void_p), ('logp_row_stride', C.c_int64),
+                ('logp_col_stride', C.c_int64), ('ref_row_stride', C.c_int64), ('ref_col_stride', C.c_int64),
+                ('weights', C.c_void_p), ('grad', C.c_void_p), ('chosen_reward', C.c_void_p),
+                ('rejected_reward', C.c_void_p), ('stats', C.c_void_p), ('beta', C.c_float),
+                ('label_smoothing', C.c_float), ('margin', C.c_float), ('kind', C.c_int), ('average', C.c_int),
+                ('denominator', C.c_double), ('grad_scale', C.c_float)]
+
+
+class TransitionDesc(C.Structure):
+    _fields_ = [('horizon', C.c_int), ('transition_dim', C.c_int), ('action_dim', C.c_int), ('observation_dim', C.c_int),
+                ('n_timesteps', C.c_int), ('clip_denoised', C.c_int), ('n_cond', C.c_int), ('cond_index', C.c_int * 4),
+                ('pred_stride', C.c_int64), ('x_stride', C.c_int64), ('x_prev_stride', C.c_int64),
+                ('posterior_log_variance', C.c_void_p), ('coef1', C.c_void_p), ('coef2', C.c_void_p),
+                ('sqrt_recip_alphas_cumprod', C.c_void_p), ('sqrt_recipm1_alphas_cumprod', C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 _VP = C.c_void_p
 SIGNATURES = {
@@ -104,6 +141,19 @@ SIGNATURES = {
     'trebi_trainer_accumulate': (C.c_int, [_VP, _VP, C.POINTER(_VP), _VP, _VP, C.c_int, C.c_float, _VP, _VP]),
     'trebi_trainer_step': (C.c_int, [_VP, C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int, C.c_float,
                                      _VP]),
+    'trebi_grad_set_bytes': (C.c_size_t, [C.c_int, c_i64_p]),
+    'trebi_grad_set_fill': (C.c_int, [C.c_int, C.POINTER(_VP), c_i64_p, C.POINTER(C.c_int), _VP, C.c_size_t,
+                                      C.POINTER(GradSet)]),
+    'trebi_grad_workspace_bytes': (C.c_size_t, [C.POINTER(GradSet)]),
+    'trebi_grad_norm': (C.c_int, [_VP, C.POINTER(GradSet), _VP, C.c_int, C.c_float, _VP, _VP, C.c_size_t, _VP]),
+    'trebi_grad_clip': (C.c_int, [_VP, C.POINTER(GradSet), _VP, C.c_int, C.c_float, C.c_float, _VP, _VP, _VP, C.c_size_t,
+                                  _VP]),
+    'trebi_policy_loss_workspace_bytes': (C.c_size_t, [C.POINTER(TokenDesc)]),
+    'trebi_policy_loss': (C.c_int, [_VP, C.POINTER(TokenDesc), C.POINTER(PolicyLossDesc), _VP, C.c_size_t, _VP]),
+    'trebi_preference_loss_workspace_bytes': (C.c_size_t, [C.POINTER(TokenDesc)]),
+    'trebi_preference_loss': (C.c_int, [_VP, C.POINTER(TokenDesc), C.POINTER(PreferenceLossDesc), _VP, C.c_size_t, _VP]),
+    'trebi_transition_logp': (C.c_int, [_VP, C.POINTER(TransitionDesc), _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP]),
+    'trebi_transition_logp_grad': (C.c_int, [_VP, C.POINTER(TransitionDesc), _VP, _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP]),
 }
 
 _lib = None

@@ -1,0 +1,304 @@
+"""Fine-tuning losses over log-probabilities, with their gradients, and the log-probability of a denoise transition, on the
+HIP library (trebi_policy_loss, trebi_preference_loss, trebi_transition_logp).
+
+Like the training step, these take no part in torch's autograd: a call returns the loss AND its gradient with respect to
+the log-probabilities (times grad_scale), which the caller hands on -- TrainEngine.accumulate_policy / accumulate_preference
+do so for the TemporalUnet, `logp.backward(result.grad)` does for a torch graph.  Nothing waits for the GPU, results do not
+change from run to run, and the calls can be captured into a graph.  The reference has none of these losses.
+
+Which tokens count (a token: one denoise step of a trajectory, one position of a sequence):
+    logp [rows, len]                   all of them, or with lengths= [rows] a row's first ones, or / and mask= [rows, len]
+    logp [tokens], cu_seqlens=         packed rows, row r at [cu_seqlens[r], cu_seqlens[r+1])  (and mask= [tokens])
+    logp [rows]                        rows of one token
+What stands at tokens that do not count is never used; their gradient is 0.  Inputs are float32, bfloat16 or float16 (one
+type for all log-probabilities); advantages and weights float32.
+"""
+import ctypes as C
+from collections import namedtuple
+
+import torch
+
+from . import _lib
+
+PolicyLoss = namedtuple('PolicyLoss', 'loss grad policy kl clip_fraction ratio')
+PreferenceLoss = namedtuple('PreferenceLoss', 'loss grad chosen_reward rejected_reward accuracy margin')
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_KL = {'k1': 1, 'k2': 2, 'k3': 3}
+_REDUCTIONS = {'token': 0, 'sequence': 1}
+_KINDS = {'sigmoid': 0, 'hinge': 1, 'ipo': 2}
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _check_logp(logp):
+    if not logp.is_cuda:
+        raise RuntimeError('trebi_amd losses run on an MI355X only; there is no CPU path')
+    if logp.dtype not in _DTYPES:
+        raise TypeError(f'logp has type {logp.dtype}; float32, bfloat16 and float16 are supported')
+
+
+def _like(name, v, logp):
+    """Another per-token tensor of logp's shape, type and device."""
+    if v.shape != logp.shape:
+        raise ValueError(f'{name} has shape {tuple(v.shape)}, logp {tuple(logp.shape)}')
+    if v.dtype != logp.dtype:
+        raise TypeError(f'{name} has type {v.dtype}, logp {logp.dtype}')
+    if v.device != logp.device:
+        raise RuntimeError(f'{name} is on {v.device}, logp on {logp.device}')
+    return v
+
+
+def _ints(name, v, n, device):
+    if not torch.is_tensor(v):
+        v = torch.as_tensor(v)
+    if v.shape != (n,) and n is not None or v.dim() != 1 or v.is_floating_point() or v.dtype == torch.bool:
+        raise ValueError(f'{name} must be an integer tensor of shape [{n if n is not None else "rows + 1"}], got {v.dtype} {tuple(v.shape)}')
+    return v.to(device, torch.int32).contiguous()
+
+
+def _token_desc(logp, mask, lengths, cu_seqlens):
+    """(descriptor, rows, what it points to) -- the last to be kept until the call was enqueued."""
+    dev = logp.device
+    keep = []
+    if mask is not None:
+        if mask.shape != logp.shape or mask.device != dev:
+            raise ValueError(f'mask is {tuple(mask.shape)} on {mask.device}, logp {tuple(logp.shape)} on {dev}')
+        if mask.dtype not in (torch.bool, torch.uint8):
+            mask = mask != 0
+    if cu_seqlens is not None:
+        if lengths is not None:
+            raise ValueError('lengths belong to padded rows, cu_seqlens to packed ones')
+        if logp.dim() != 1:
+            raise ValueError(f'packed logp is [tokens], got {tuple(logp.shape)}')
+        cu = _ints('cu_seqlens', cu_seqlens, None, dev)
+        if cu.numel() < 1:
+            raise ValueError('cu_seqlens has rows + 1 entries')
+        if mask is not None:
+            mask = mask.contiguous()
+        keep += [cu, mask]
+        rows = cu.numel() - 1
+        d = _lib.TokenDesc(rows, logp.numel(), 1, None, cu.data_ptr(), None if mask is None else mask.data_ptr(), 0, 1)
+        return d, rows, keep
+    rows, length = logp.shape
+    at = None
+    if lengths is not None:
+        at = _ints('lengths', lengths, rows, dev)
+    keep += [at, mask]
+    ms = (0, 1) if mask is None else mask.stride()
+    d = _lib.TokenDesc(rows, length, 0, None if at is None else at.data_ptr(), None,
+                       None if mask is None else mask.data_ptr(), ms[0], ms[1])
+    return d, rows, keep
+
+
+def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=None, clip=0.2,
+                clip_high=None, dual_clip=None, kl_coef=0.0, kl='k3', reduction='token', denominator=None, grad_scale=1.0,
+                want_grad=True, per_token=None):
+    """Clipped policy loss with a KL term:
+
+        rho = exp(logp - logp_old)                       (logp_old None: on-policy, rho = 1)
+        pg  = -min(rho A, clamp(rho, 1 - clip, 1 + clip_high) A),  with dual_clip c at most c |A| where A < 0
+        kl  = 'k1': logp - ref | 'k2': (logp - ref)^2 / 2 | 'k3': exp(ref - logp) - (ref - logp) - 1    (no logp_ref: 0)
+        loss = sum_i w_i (pg_i + kl_coef kl_i)
+
+    w: 1 / valid tokens ('token'), 1 / (rows that are not empty * the row's valid tokens) ('sequence'), or 1 / denominator
+    where that is given (data-parallel: the global count).  Nothing valid: loss 0.  advantages: one a row or one a token, told
+    by their shape, or by per_token (packed rows may be as many as tokens; then one a row is assumed).
+    Returns PolicyLoss(loss, grad [like logp] | None, policy, kl, clip_fraction, ratio); loss = policy + kl_coef * kl, and
+    clip_fraction / ratio are means over the valid tokens."""
+    _check_logp(logp)
+    shape, dev = logp.shape, logp.device
+    if logp.dim() == 1 and cu_seqlens is None:
+        one = lambda v: v if v is None or v.dim() != 1 else v[:, None]
+        if lengths is not None:
+            raise ValueError('rows of one token take no lengths')
+        logp, logp_old, logp_ref, mask = one(logp), one(logp_old), one(logp_ref), one(mask)
+    if logp.dim() != (2 if cu_seqlens is None else 1):
+        raise ValueError(f'logp is [rows, len], [rows] or (with cu_seqlens) [tokens], got {tuple(shape)}')
+    if kl not in _KL or reduction not in _REDUCTIONS:
+        raise ValueError(f"kl must be 'k1', 'k2' or 'k3' and reduction 'token' or 'sequence', got {kl!r}, {reduction!r}")
+    if logp_old is not None:
+        _like('logp_old', logp_old, logp)
+    if logp_ref is not None:
+        _like('logp_ref', logp_ref, logp)
+    d, rows, keep = _token_desc(logp, mask, lengths, cu_seqlens)
+    if advantages.dtype != torch.float32 or advantages.device != dev:
+        raise TypeError(f'advantages must be float32 on {dev}, got {advantages.dtype} on {advantages.device}')
+    packed = cu_seqlens is not None
+    if packed:
+        logp = logp.contiguous()
+        logp_old = None if logp_old is None else logp_old.contiguous()
+        logp_ref = None if logp_ref is None else logp_ref.contiguous()
+        strides = [(0, 1)] * 3
+        if advantages.shape == (rows,) and not per_token:
+            adv_stride = (advantages.stride(0), 0)
+        elif advantages.shape == logp.shape and per_token is not False:
+            advantages, adv_stride = advantages.contiguous(), (0, 1)
+        else:
+            raise ValueError(f'advantages must be [{rows}] or {tuple(logp.shape)}, got {tuple(advantages.shape)}')
+    else:
+        strides = [logp.stride(), (0, 1) if logp_old is None else logp_old.stride(), (0, 1) if logp_ref is None else logp_ref.stride()]
+        if advantages.shape in ((rows,), (rows, 1)) and (not per_token or logp.shape[1] == 1):
+            adv_stride = (advantages.stride(0), 0)
+        elif advantages.shape == logp.shape and per_token is not False:
+            adv_stride = advantages.stride()                        # (column stride 0: one a row, expanded)
+        else:
+            raise ValueError(f'advantages must be [{rows}] or {tuple(logp.shape)}, got {tuple(advantages.shape)}')
+    grad = torch.empty(logp.shape, dtype=logp.dtype, device=dev) if want_grad else None
+    if rows == 0 or logp.numel() == 0:
+        z = torch.zeros(5, device=dev).unbind()
+        return PolicyLoss(z[0], None if grad is None else grad.zero_().reshape(shape), *z[1:])
+    stats = torch.empty(5, device=dev)
+    lib = _lib.lib()
+    ws = torch.empty(lib.trebi_policy_loss_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=dev)
+    q = _lib.PolicyLossDesc(
+        _DTYPES[logp.dtype], logp.data_ptr(), None if logp_old is None else logp_old.data_ptr(),
+        None if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1], *strides[2], advantages.data_ptr(),
+        *adv_stride, None if grad is None else grad.data_ptr(), stats.data_ptr(), clip, clip if clip_high is None else clip_high,
+        0.0 if dual_clip is None else dual_clip, kl_coef, _KL[kl], _REDUCTIONS[reduction] if denominator is None else 2,
+        0.0 if denominator is None else denominator, grad_scale)
+    _lib.check(lib.trebi_policy_loss(_lib.ctx(dev.index or 0), C.byref(d), C.byref(q), ws.data_ptr(), ws.numel(), _stream(dev)))
+    loss, policy, klv, cut, ratio = stats.unbind()
+    return PolicyLoss(loss, grad if grad is None or grad.shape == shape else grad.reshape(shape), policy, klv, cut, ratio)
+
+
+def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=None, weights=None, beta=0.1, kind='sigmoid',
+                    label_smoothing=0.0, margin=0.0, average=False, denominator=None, grad_scale=1.0, want_grad=True):
+    """Preference loss over paired log ratios.  Of 2 P rows, row k is preferred to row k + P.
+
+        D_r = sum over the row's valid tokens of logp - logp_ref   (no logp_ref: logp; average: divided by their number)
+        h = D_k - D_{k+P},  z = beta h - margin
+        'sigmoid': -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing
+        'hinge':   max(0, 1 - z)
+        'ipo':     (z / beta - 1 / (2 beta))^2
+        loss = sum_k weights[k] l_k / P     (denominator instead of P where given; data-parallel: the global number of pairs)
+
+    A pair with an empty row gives neither loss nor gradient.  Returns PreferenceLoss(loss, grad [like logp] | None,
+    chosen_reward [P], rejected_reward [P] (beta D), accuracy (share of the pairs that count with h > 0), margin (their
+    mean z))."""
+    _check_logp(logp)
+    shape, dev = logp.shape, logp.device
+    if logp.dim() == 1 and cu_seqlens is None:
+        one = lambda v: v if v is None or v.dim() != 1 else v[:, None]
+        if lengths is not None:
+            raise ValueError('rows of one token take no lengths')
+        logp, logp_ref, mask = one(logp), one(logp_ref), one(mask)
+    if logp.dim() != (2 if cu_seqlens is None else 1):
+        raise ValueError(f'logp is [2 P, len], [2 P] or (with cu_seqlens) [tokens], got {tuple(shape)}')
+    if kind not in _KINDS:
+        raise ValueError(f"kind must be 'sigmoid', 'hinge' or 'ipo', got {kind!r}")
+    if label_smoothing and kind != 'sigmoid':
+        label_smoothing = 0.0                                       # the other kinds have no smoothed form
+    if logp_ref is not None:
+        _like('logp_ref', logp_ref, logp)
+    d, rows, keep = _token_desc(logp, mask, lengths, cu_seqlens)
+    if rows % 2:
+        raise ValueError(f'{rows} rows: chosen and rejected rows come in pairs')
+    P = rows // 2
+    if weights is not None:
+        if weights.shape != (P,) or weights.dtype != torch.float32 or weights.device != dev:
+            raise ValueError(f'weights must be float32 [{P}] on {dev}, got {weights.dtype} {tuple(weights.shape)} on {weights.device}')
+        weights = weights.contiguous()
+    if cu_seqlens is not None:
+        logp = logp.contiguous()
+        logp_ref = None if logp_ref is None else logp_ref.contiguous()
+        strides = [(0, 1)] * 2
+    else:
+        strides = [logp.stride(), (0, 1) if logp_ref is None else logp_ref.stride()]
+    grad = torch.empty(logp.shape, dtype=logp.dtype, device=dev) if want_grad else None
+    if P == 0:
+        z = torch.zeros(3, device=dev).unbind()
+        e = torch.empty(0, device=dev)
+        return PreferenceLoss(z[0], None if grad is None else grad.zero_().reshape(shape), e, e.clone(), z[1], z[2])
+    out = torch.empty(2 * P + 3, device=dev)
+    chosen, rejected, stats = out[:P], out[P:2 * P], out[2 * P:]
+    lib = _lib.lib()
+    ws = torch.empty(lib.trebi_preference_loss_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=dev)
+    at = out.data_ptr()
+    q = _lib.PreferenceLossDesc(
+        _DTYPES[logp.dtype], logp.data_ptr() or None, None if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1],
+        None if weights is None else weights.data_ptr(), None if grad is None else grad.data_ptr() or None, at, at + 4 * P,
+        at + 8 * P, beta, label_smoothing, margin, _KINDS[kind], int(bool(average)), 0.0 if denominator is None else denominator,
+        grad_scale)
+    _lib.check(lib.trebi_preference_loss(_lib.ctx(dev.index or 0), C.byref(d), C.byref(q), ws.data_ptr(), ws.numel(), _stream(dev)))
+    loss, acc, mz = stats.unbind()
+    return PreferenceLoss(loss, grad if grad is None or grad.shape == shape else grad.reshape(shape), chosen, rejected, acc, mz)
+
+
+# ------------------------------------------------------------------------------------------- denoise transitions
+def _rows(name, v, shape, device):
+    """float32 [B, H, D] whose candidates are contiguous (a slice of a chain keeps its stride), copied otherwise."""
+    if v.shape != shape or v.device != device:
+        raise ValueError(f'{name} is {tuple(v.shape)} on {v.device}, expected {tuple(shape)} on {device}')
+    if v.dtype != torch.float32:
+        raise TypeError(f'{name} must be float32, got {v.dtype}')
+    if v.stride(2) != 1 and shape[2] > 1 or v.stride(1) != shape[2] and shape[1] > 1:
+        v = v.contiguous()
+    return v, v.stride(0)
+
+
+def _transition(model, pred, x, x_prev, t, cond_keys):
+    dev = pred.device
+    if dev.type != 'cuda':
+        raise RuntimeError('trebi_amd computes transition log-probabilities on an MI355X only; there is no CPU path')
+    if pred.dim() != 3 or pred.shape[2] != model.transition_dim:
+        raise ValueError(f'pred must be [batch, horizon, {model.transition_dim}], got {tuple(pred.shape)}')
+    B, H, D = pred.shape
+    pred, ps = _rows('pred', pred, pred.shape, dev)
+    x, xs = _rows('x', x, pred.shape, dev)
+    x_prev, qs = _rows('x_prev', x_prev, pred.shape, dev)
+    if not torch.is_tensor(t):
+        t = torch.as_tensor(t)
+    if t.dim() == 0:
+        t = t.expand(B)
+    if t.shape != (B,) or t.is_floating_point():
+        raise ValueError(f't must be [{B}] integers, got {t.dtype} {tuple(t.shape)}')
+    if not t.is_cuda and B and not (0 <= int(t.min()) and int(t.max()) < model.n_timesteps):
+        raise RuntimeError(f'timesteps must lie in [0, {model.n_timesteps})')
+    t = t.to(dev, torch.int64).contiguous()
+    keys = sorted(int(k) for k in cond_keys)
+    if len(keys) > 4:
+        raise RuntimeError('at most 4 conditioned timesteps are supported')
+    names = ['posterior_log_variance_clipped', 'posterior_mean_coef1', 'posterior_mean_coef2']
+    if model.predict_epsilon:
+        names += ['sqrt_recip_alphas_cumprod', 'sqrt_recipm1_alphas_cumprod']
+    tabs = [getattr(model, n) for n in names]
+    for n, tab in zip(names, tabs):
+        if tab.device != dev or tab.dtype != torch.float32 or tab.shape != (model.n_timesteps,) or not tab.is_contiguous():
+            raise RuntimeError(f'{n} must be a contiguous float32 [{model.n_timesteps}] on {dev}')
+    ptrs = [tab.data_ptr() for tab in tabs] + [None] * (5 - len(tabs))
+    d = _lib.TransitionDesc(H, D, model.action_dim, model.observation_dim, model.n_timesteps, int(bool(model.clip_denoised)),
+                            len(keys), (C.c_int * 4)(*keys), ps, xs, qs, *ptrs)
+    return d, pred, x, x_prev, t
+
+
+def transition_log_prob(model, pred, x, x_prev, t, cond_keys=(0,)):
+    """log p(x_prev | x) [B] of the reverse step at timesteps t (GaussianDiffusion.p_mean_variance and the draw of the sample
+    functions, diffusion.py:153-185), given the net's output `pred` = model.model(x, cond, t); `model` is the
+    GaussianDiffusion.  Elements that a condition overwrites (observation part of the rows cond_keys) do not count, and a
+    transition at t = 0, which adds no noise, has log-probability 0.  x and x_prev may be slices of a returned chain.  (A CUDA
+    t is not checked here: the kernels cut it to the tables.)"""
+    d, pred, x, x_prev, t = _transition(model, pred, x, x_prev, t, cond_keys)
+    B = pred.shape[0]
+    logp = torch.empty(B, device=pred.device)
+    if B:
+        _lib.check(_lib.lib().trebi_transition_logp(_lib.ctx(pred.device.index or 0), C.byref(d), pred.data_ptr(), x.data_ptr(),
+                                                    x_prev.data_ptr(), t.data_ptr(), B, logp.data_ptr(), _stream(pred.device)))
+    return logp
+
+
+def transition_log_prob_grad(model, pred, x, x_prev, t, grad, cond_keys=(0,)):
+    """grad[b] * d transition_log_prob[b] / d pred, [B, H, D]; `grad`: float32 [B], d loss / d log-probability."""
+    d, pred, x, x_prev, t = _transition(model, pred, x, x_prev, t, cond_keys)
+    B = pred.shape[0]
+    if grad.shape != (B,) or grad.dtype != torch.float32 or grad.device != pred.device:
+        raise ValueError(f'grad must be float32 [{B}] on {pred.device}, got {grad.dtype} {tuple(grad.shape)} on {grad.device}')
+    grad = grad.contiguous()
+    out = torch.empty(pred.shape, device=pred.device)
+    if B:
+        _lib.check(_lib.lib().trebi_transition_logp_grad(
+            _lib.ctx(pred.device.index or 0), C.byref(d), pred.data_ptr(), x.data_ptr(), x_prev.data_ptr(), t.data_ptr(),
+            grad.data_ptr(), B, out.data_ptr(), _stream(pred.device)))
+    return out
