@@ -354,7 +354,7 @@ typedef enum { TREBI_F32 = 0, TREBI_BF16 = 1, TREBI_F16 = 2 } trebi_dtype;
  * bytes, which the caller copies to the device (256-byte aligned) and keeps, with `out`, while the tensors stay where
  * they are.  trebi_grad_clip scales in place, or with `out` leaves the gradients alone and writes the scaled values back
  * to back (in the tensors' order) as `total` float32.  norm_out: dev [1], nullable in trebi_grad_clip. */
-typedef struct { int n_tensors, n_chunks; int64_t total; } trebi_grad_set;
+typedef struct { int n_tensors, n_chunks; int64_t total, bytes; } trebi_grad_set;
 size_t trebi_grad_set_bytes(int n_tensors, const int64_t* numels);
 int trebi_grad_set_fill(int n_tensors, const void* const* tensors, const int64_t* numels, const int* dtypes, void* host_table,
                         size_t table_bytes, trebi_grad_set* out);

@@ -1,4 +1,4 @@
-// Kernel arguments and launchers of the fine-tuning operators (gradnorm.hip, losses.hip), shared with the host side
+// Kernel arguments and launchers of the fine-tuning operators (gradnorm.hip, policy.hip, pairs.hip, transition.hip), shared with the host side
 // (finetune.inl).
 #pragma once
 #include <hip/hip_runtime.h>
@@ -7,20 +7,19 @@
 namespace trebi {
 
 // ---- global gradient norm over many tensors ------------------------------------------------------------------
-// The set's table lives in device memory: the tensors, then the chunks they are cut into (one chunk = consecutive
-// elements of one tensor; a workgroup walks whole chunks).
-struct GradTensor { void* p; long long numel; long long out_off; int dtype; int pad; };
-struct GradChunk { long long off; int tensor; int len; };
-constexpr int GRAD_BLOCKS = 2048;          // partial sums a launch may leave, = workgroups: 8 of 256 threads on each CU
+// The set's table lives in device memory: the chunks that the tensors are cut into (a chunk: consecutive elements of one
+// tensor).  Workgroup w takes the chunks w, w + n_blocks, ..., so that at any moment the workgroups read and write one
+// moving window of memory.
+struct GradChunk { void* p; long long out_off; int len; int dtype; };
+constexpr int GRAD_BLOCKS = 2048;          // workgroups of 256 threads at most: 8 on each CU
 struct GradP {
-  const GradTensor* tensors;
   const GradChunk* chunks;
-  int n_chunks, norm_type;                 // 0 two-norm, 1 one-norm, 2 largest magnitude
+  int n_chunks, n_blocks, norm_type;       // 0 two-norm, 1 one-norm, 2 largest magnitude
+  int stream_loads, stream_stores;         // past the caches: nothing will read it from there
   float grad_scale, max_norm;
   float* out;                              // flat float32 copy, or null: in place
   float* norm_out;                         // [1] or null
-  double* part;                            // [n_part]
-  int n_part;
+  double* part;                            // [n_blocks]
 };
 hipError_t launch_grad_partials(const GradP& p, hipStream_t st);
 hipError_t launch_grad_finish(const GradP& p, float* coef_out, hipStream_t st);     // norm and (coef_out) the factor
@@ -37,7 +36,7 @@ struct TokenP {
 };
 struct NormPart { long long tokens, rows; };
 constexpr int COUNT_BLOCKS = 256;          // partial counts
-constexpr int LOSS_PARTS = 2048;           // partial sums a loss kernel may leave
+constexpr int LOSS_PARTS = 1280;          // workgroups of the policy loss at most: the 5 that fit on each CU at once
 constexpr int LOSS_VALS = 5;
 
 struct PolicyP {
@@ -48,18 +47,20 @@ struct PolicyP {
   long long ars, acs;                      // acs 0: one advantage a row
   void* grad;                              // contiguous, the type of lp; or null
   double hi, lo, dual;                     // borders of the log ratio
+  float fhi, flo, fdual;                   // the same, rounded
   float vhi, vlo, vdual;                   // the ratio taken beyond them
   float kl_coef;
   int kl, mode;                            // 1..3; 0 token mean, 1 mean over sequences, 2 a given denominator
   double fixed;                            // mode 2: 1 / denominator; else > 0: 1 / count known on the host, 0: from `np`
   float gscale;
   NormPart* np;
-  int nnp;                                 // partial counts written (0: none needed)
+  int nnp;                                 // partial counts written (0: none, the kernel counts the rows itself)
   int* counts;                             // [rows] valid tokens of a row under a mask, or null
-  double* part;                            // [LOSS_PARTS][LOSS_VALS]
+  double* part;                            // [LOSS_VALS][LOSS_PARTS]
+  double* weight;                          // the weight, from the loss kernel to the one that finishes
   float* stats;                            // [5]
   long long per;                           // tokens of a workgroup
-  int flat;                                // every view is contiguous: vector loads across rows
+  int flat;                                // every view is contiguous and rows are not tiny: vector loads across rows
 };
 hipError_t launch_token_counts(const PolicyP& p, hipStream_t st);
 hipError_t launch_policy(const PolicyP& p, int dtype, int blocks, hipStream_t st);

@@ -1,6 +1,6 @@
 // finetune.inl -- host side of the fine-tuning operators (included at the end of trebi.hip): argument checks and launch
-// shapes of the gradient norm (gradnorm.hip), the policy and preference losses and the transition log-probability
-// (losses.hip).  Nothing here allocates, synchronises or keeps state: tables and workspaces are the caller's.
+// shapes of the gradient norm (gradnorm.hip), the policy loss (policy.hip), the preference loss (pairs.hip) and the
+// transition log-probability (transition.hip).  Nothing here allocates, synchronises or keeps state: tables and workspaces are the caller's.
 #include "finetune.h"
 
 namespace {
@@ -22,19 +22,21 @@ struct DeviceGuard {
   DeviceGuard on_device((ctx)->device);   \
   HIPCHK(on_device.err)
 
-// Elements of a chunk: about four chunks for each of the workgroups, so that ends of tensors even out, and never
-// less than a workgroup reads at one go four times over.
+size_t al256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Elements of a chunk: whole turns of a workgroup (256 threads x 8 loads of 16 bytes: 16384 16-bit or 8192 32-bit elements),
+// about 8 chunks a workgroup of a large set; smaller sets are cut finer, so that they reach every CU.
 long long grad_chunk(long long total) {
-  const long long per = (total + 4 * GRAD_BLOCKS - 1) / (4 * GRAD_BLOCKS);
-  return std::min<long long>(std::max<long long>((per + 4095) / 4096 * 4096, 4096), 1 << 28);
+  const long long per = (total + 8 * GRAD_BLOCKS - 1) / (8 * GRAD_BLOCKS);
+  if (per > 4096) return std::min<long long>((per + 16383) / 16384 * 16384, 1 << 28);
+  return total > 2048 * 1024 ? 4096 : 2048;
 }
-size_t grad_tensors_bytes(int n) { return ((size_t)n * sizeof(GradTensor) + 255) / 256 * 256; }
 
 int grad_totals(int n, const int64_t* numels, long long* total, long long* chunks) {
   if (n < 1 || !numels) return fail(TREBI_BAD_ARG, "at least one tensor is needed");
   *total = 0;
   for (int i = 0; i < n; ++i) {
-    if (numels[i] < 0) return fail(TREBI_BAD_ARG, "tensor %d has a negative size", i);
+    if (numels[i] < 0 || numels[i] > (1ll << 48)) return fail(TREBI_BAD_ARG, "tensor %d has a bad size", i);
     *total += numels[i];
   }
   const long long c = grad_chunk(*total);
@@ -44,6 +46,10 @@ int grad_totals(int n, const int64_t* numels, long long* total, long long* chunk
   return 0;
 }
 
+// From this many bytes on the 256 MB cache cannot hand a set from one kernel to the next: such sets are read (for the norm
+// alone) and written past the caches.
+constexpr long long GRAD_STREAM = 256ll << 20;
+
 int grad_args(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float grad_scale, void* ws,
               size_t ws_bytes, GradP* p) {
   if (!ctx || !set || !table || !ws) return fail(TREBI_BAD_ARG, "null argument");
@@ -52,17 +58,15 @@ int grad_args(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int 
   if (!(grad_scale >= 0.f)) return fail(TREBI_BAD_ARG, "grad_scale must not be negative");
   if (ws_bytes < trebi_grad_workspace_bytes(set))
     return fail(TREBI_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", ws_bytes, trebi_grad_workspace_bytes(set));
-  p->tensors = (const GradTensor*)table;
-  p->chunks = (const GradChunk*)((const char*)table + grad_tensors_bytes(set->n_tensors));
+  p->chunks = (const GradChunk*)table;
   p->n_chunks = set->n_chunks;
+  const int rounds = std::max(1, (set->n_chunks + GRAD_BLOCKS - 1) / GRAD_BLOCKS);    // the same number of chunks for every workgroup
+  p->n_blocks = std::max(1, (set->n_chunks + rounds - 1) / rounds);
   p->norm_type = norm_type;
   p->grad_scale = grad_scale;
   p->part = (double*)ws;
-  p->n_part = std::max(1, std::min(set->n_chunks, GRAD_BLOCKS));
   return 0;
 }
-
-size_t al256(size_t n) { return (n + 255) / 256 * 256; }
 
 int token_args(const trebi_token_desc& d, TokenP* t) {
   if (d.rows < 0 || d.len < 0 || d.rows > (1ll << 40) || d.len > (1ll << 40)) return fail(TREBI_BAD_SHAPE, "bad number of rows or tokens");
@@ -90,17 +94,17 @@ int token_args(const trebi_token_desc& d, TokenP* t) {
 
 // policy workspace: partial counts, partial sums, a count for each row
 size_t policy_bytes(const trebi_token_desc& d) {
-  return al256(COUNT_BLOCKS * sizeof(NormPart)) + al256(LOSS_PARTS * LOSS_VALS * sizeof(double)) +
+  return al256(COUNT_BLOCKS * sizeof(NormPart)) + al256((LOSS_PARTS * LOSS_VALS + 1) * sizeof(double)) +
          (d.mask ? al256((size_t)d.rows * sizeof(int)) : 0);
 }
 
-constexpr int PAIR_BLOCKS = LOSS_PARTS;
+constexpr int PAIR_BLOCKS = 2048;
 // Rows are split over workgroups where whole pairs would leave the card idle: fewer pairs than 2 a CU, and rows of
 // more than one turn of a workgroup.  (Lengths on the device do not matter for the choice, nor for the result.)
 int pair_splits(const trebi_token_desc& d) {
   const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len;
   if (d.rows / 2 >= 512 || len <= 4096) return 0;
-  return (int)std::max<long long>(1, std::min<long long>(LOSS_PARTS / d.rows, (len + 4095) / 4096));
+  return (int)std::max<long long>(1, std::min<long long>(PAIR_BLOCKS / d.rows, (len + 4095) / 4096));
 }
 size_t pair_bytes(const trebi_token_desc& d) {
   const int s = pair_splits(d);
@@ -115,7 +119,7 @@ size_t pair_bytes(const trebi_token_desc& d) {
 extern "C" size_t trebi_grad_set_bytes(int n_tensors, const int64_t* numels) {
   long long total, chunks;
   if (grad_totals(n_tensors, numels, &total, &chunks)) return 0;
-  return grad_tensors_bytes(n_tensors) + al256((size_t)std::max<long long>(chunks, 1) * sizeof(GradChunk));
+  return al256((size_t)std::max<long long>(chunks, 1) * sizeof(GradChunk));
 }
 
 extern "C" int trebi_grad_set_fill(int n_tensors, const void* const* tensors, const int64_t* numels, const int* dtypes,
@@ -124,6 +128,11 @@ extern "C" int trebi_grad_set_fill(int n_tensors, const void* const* tensors, co
   if (!tensors || !dtypes || !host_table || !out) return fail(TREBI_BAD_ARG, "null argument");
   if (int e = grad_totals(n_tensors, numels, &total, &chunks)) return e;
   if (table_bytes < trebi_grad_set_bytes(n_tensors, numels)) return fail(TREBI_WORKSPACE_TOO_SMALL, "table of %zu bytes", table_bytes);
+  for (int i = 0; i < n_tensors; ++i) {
+    if (dtypes[i] < 0 || dtypes[i] > 2) return fail(TREBI_BAD_ARG, "tensor %d has an unknown type %d", i, dtypes[i]);
+    const size_t size = dtypes[i] == TREBI_F32 ? 4 : 2;
+    if (numels[i] && (!tensors[i] || (uintptr_t)tensors[i] % size)) return fail(TREBI_BAD_ARG, "tensor %d is null or not aligned to its type", i);
+  }
   // a byte of two tensors would be scaled twice, by two workgroups at once
   try {
     std::vector<std::pair<uintptr_t, uintptr_t>> span;
@@ -136,20 +145,20 @@ extern "C" int trebi_grad_set_fill(int n_tensors, const void* const* tensors, co
     return fail(TREBI_HIP_ERROR, "out of host memory: %s", e.what());
   }
   const long long c = grad_chunk(total);
-  GradTensor* t = (GradTensor*)host_table;
-  GradChunk* ch = (GradChunk*)((char*)host_table + grad_tensors_bytes(n_tensors));
-  long long at = 0;
+  GradChunk* ch = (GradChunk*)host_table;
+  *ch = GradChunk{nullptr, 0, 0, 0};                       // (a set of empty tensors)
+  long long at = 0, bytes = 0;
   for (int i = 0; i < n_tensors; ++i) {
-    if (dtypes[i] < 0 || dtypes[i] > 2) return fail(TREBI_BAD_ARG, "tensor %d has an unknown type %d", i, dtypes[i]);
     const size_t size = dtypes[i] == TREBI_F32 ? 4 : 2;
-    if (numels[i] && (!tensors[i] || (uintptr_t)tensors[i] % size)) return fail(TREBI_BAD_ARG, "tensor %d is null or not aligned to its type", i);
-    t[i] = GradTensor{(void*)tensors[i], (long long)numels[i], at, dtypes[i], 0};
+    for (long long o = 0; o < numels[i]; o += c)
+      *ch++ = GradChunk{(char*)tensors[i] + o * size, at + o, (int)std::min<long long>(c, numels[i] - o), dtypes[i]};
     at += numels[i];
-    for (long long o = 0; o < numels[i]; o += c) *ch++ = GradChunk{o, i, (int)std::min<long long>(c, numels[i] - o)};
+    bytes += numels[i] * size;
   }
   out->n_tensors = n_tensors;
   out->n_chunks = (int)chunks;
   out->total = total;
+  out->bytes = bytes;
   return 0;
 }
 
@@ -161,6 +170,7 @@ extern "C" int trebi_grad_norm(trebi_ctx* ctx, const trebi_grad_set* set, const 
   if (int e = grad_args(ctx, set, table, norm_type, grad_scale, workspace, workspace_bytes, &p)) return e;
   if (!norm_out) return fail(TREBI_BAD_ARG, "norm_out is null");
   p.norm_out = norm_out;
+  p.stream_loads = set->bytes > GRAD_STREAM;
   ON_DEVICE(ctx);
   HIPCHK(launch_grad_partials(p, (hipStream_t)stream));
   HIPCHK(launch_grad_finish(p, nullptr, (hipStream_t)stream));
@@ -176,6 +186,7 @@ extern "C" int trebi_grad_clip(trebi_ctx* ctx, const trebi_grad_set* set, const 
   p.max_norm = max_norm;
   p.out = out;
   p.norm_out = norm_out;
+  p.stream_stores = set->bytes + (out ? 4 * set->total : 0) > GRAD_STREAM;
   ON_DEVICE(ctx);
   HIPCHK(launch_grad_partials(p, (hipStream_t)stream));
   HIPCHK(launch_grad_scale(p, (hipStream_t)stream));
@@ -211,6 +222,7 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
   p.hi = std::log1p((double)d->clip_high);
   p.lo = d->clip_low < 1.f ? std::log1p(-(double)d->clip_low) : -INFINITY;
   p.dual = d->dual_clip > 1.f ? std::log((double)d->dual_clip) : INFINITY;
+  p.fhi = (float)p.hi; p.flo = (float)p.lo; p.fdual = (float)p.dual;
   p.vhi = (float)(1.0 + (double)d->clip_high);
   p.vlo = (float)(1.0 - (double)d->clip_low);
   p.vdual = d->dual_clip;
@@ -233,27 +245,30 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
   const bool flat_mask = !t.mask || (t.packed ? t.mcs == 1 : t.mcs == 1 && t.mrs == L);
   p.flat = flat_lp && flat_old && flat_ref && flat_adv && flat_mask;
   if (t.packed && !p.flat) return fail(TREBI_UNSUPPORTED_CONFIG, "packed tensors are contiguous");
+  // rows shorter than the tokens of a thread (packed: than 8 on average) go token by token: these would lie in many rows
+  const int pack = d->dtype == TREBI_F32 ? 4 : 8;
+  if (t.packed ? t.n < 8 * t.rows : L < pack) p.flat = 0;
   const bool all = !t.packed && !t.lengths && !t.mask;
   if (p.mode == 2) p.fixed = 1.0 / d->denominator;
   else if (all && !empty) p.fixed = 1.0 / (double)(p.mode == 0 ? t.n : t.rows);
   char* w = (char*)workspace;
   p.np = (NormPart*)w; w += al256(COUNT_BLOCKS * sizeof(NormPart));
-  p.part = (double*)w; w += al256(LOSS_PARTS * LOSS_VALS * sizeof(double));
+  p.part = (double*)w; w += al256((LOSS_PARTS * LOSS_VALS + 1) * sizeof(double));
+  p.weight = p.part + LOSS_PARTS * LOSS_VALS;
   p.counts = t.mask && p.mode == 1 ? (int*)w : nullptr;
   hipStream_t st = (hipStream_t)stream;
   ON_DEVICE(ctx);
-  if (!empty && (p.fixed == 0.0 || p.counts)) {
-    p.nnp = (int)std::min<long long>(COUNT_BLOCKS, std::max<long long>(1, t.mask ? t.rows : (t.rows + 255) / 256));
+  // One workgroup does it all up to 4096 tokens (at most 4 turns): a call of this size is bound by its launches.
+  const long long turn = 256 * pack, turns = (t.n + turn - 1) / turn;
+  const long long per = t.n <= 4096 ? std::max<long long>(turns, 1) : (turns + LOSS_PARTS - 1) / LOSS_PARTS;
+  const int blocks = (int)((turns + per - 1) / per);
+  p.per = per * turn;
+  if (!empty && (p.counts || (p.fixed == 0.0 && (blocks > 1 || t.mask || t.rows > 4096)))) {
+    p.nnp = (int)(t.mask ? std::min<long long>(COUNT_BLOCKS, t.rows) : std::min<long long>(16, (t.rows + 255) / 256));
     HIPCHK(launch_token_counts(p, st));
   }
-  int blocks = 0;
-  if (!empty) {
-    const long long turns = (t.n + 2047) / 2048;                       // 256 threads x 8 tokens
-    const long long per = (turns + LOSS_PARTS - 1) / LOSS_PARTS;
-    p.per = per * 2048;
-    blocks = (int)((turns + per - 1) / per);
-    HIPCHK(launch_policy(p, d->dtype, blocks, st));
-  }
+  if (!empty) HIPCHK(launch_policy(p, d->dtype, blocks, st));
+  if (blocks == 1) return 0;
   HIPCHK(launch_policy_finish(p, blocks, st));
   return 0;
 }
@@ -298,13 +313,13 @@ extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tok
     HIPCHK(launch_pairs_split(p, d->dtype, st));
   } else {
     const long long len = p.tk.packed ? (p.tk.n + p.tk.rows - 1) / p.tk.rows : p.tk.len;
-    p.group = len <= 128 ? 16 : len <= 1024 ? 64 : 256;
+    p.group = len <= 128 ? 16 : len <= 512 ? 64 : 256;            // at most two turns of 16 tokens a thread, on average
     const long long per = 256 / p.group;
     const int blocks = (int)std::min<long long>(PAIR_BLOCKS, (p.pairs + per - 1) / per);
     p.nparts = blocks;
     HIPCHK(launch_pairs_whole(p, d->dtype, blocks, st));
   }
-  HIPCHK(launch_pairs_finish(p, st));
+  if (p.splits || p.nparts > 1) HIPCHK(launch_pairs_finish(p, st));
   return 0;
 }
 

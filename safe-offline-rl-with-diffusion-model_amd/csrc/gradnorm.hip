@@ -4,11 +4,10 @@
 //   out = c * g                           s: the factor that takes a loss scale off (1 / loss scale)
 //
 // Bound by memory: every gradient is read once for the norm and once more (partly still in the 256 MB cache) for the
-// scaled copy.  The tensors are cut into chunks on the host; a workgroup walks chunks, so that 400 tensors cost the
-// same two launches as one.  The sum is taken in float64: the card converts and adds doubles at half the float rate,
-// several times faster than HBM delivers, and then no length and no magnitude (1e-30 .. 1e30) loses digits or
-// overflows.  Each workgroup leaves one partial sum; the kernel that scales adds the partials up itself, every
-// workgroup in the same order, so no atomics, no order that changes from run to run, and no third launch.
+// scaled copy.  The tensors are cut into chunks on the host and the workgroups walk chunks, so that 400 tensors cost the same
+// two launches as one.  The sum is held in float64: no length and no magnitude (1e-30 .. 1e30) loses digits or overflows.
+// Each workgroup leaves one partial sum; the kernel that scales adds the partials up itself, every workgroup in the same
+// order, so no atomics, no order that changes from run to run, and no third launch.
 #include "finetune.h"
 #include "tokens.h"
 
@@ -37,62 +36,106 @@ __device__ __forceinline__ double block_join(double a, double* lds) {
   return a;
 }
 
-template <int NORM, typename T>
-__device__ __forceinline__ double chunk_norm(const T* p, int len) {
-  constexpr int V = 16 / sizeof(T);                   // one 16-byte load
-  double a0 = 0, a1 = 0;
-  int i = threadIdx.x * V;
-  for (; i + 3 * 256 * V + V <= len; i += 4 * 256 * V) {   // four loads in flight
-    float v[4][V];
+// V elements joined to the running values.  Pairs are formed in float32 (one rounding each, 2^-24 of the pair) and added in
+// float64: half the float64 work of adding every element, which bfloat16 gradients would otherwise wait for.  Squares
+// that leave the middle of float32's range are formed in float64 instead.
+template <int NORM, int V>
+__device__ __forceinline__ void join_vec(const float* v, double* a0, double* a1) {
+  if (NORM == 2) {
+    float m = fabsf(v[0]);
+    bool nan = v[0] != v[0];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load_vec<V>(p + i + u * 256 * V, v[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        a0 = norm_acc<NORM>(a0, v[u][e]);
-        a1 = norm_acc<NORM>(a1, v[u][e + 1]);
-      }
-  }
-  for (; i < len; i += 256 * V) {
-    if (i + V <= len) {
-      float v[V];
-      load_vec<V>(p + i, v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) a0 = norm_acc<NORM>(a0, v[e]);
-    } else {
-      for (int e = i; e < len; ++e) a0 = norm_acc<NORM>(a0, load_one(p + e));
+    for (int e = 1; e < V; ++e) {
+      m = fmaxf(m, fabsf(v[e]));
+      nan = nan || v[e] != v[e];
     }
+    *a0 = norm_join<2>(*a0, nan ? __builtin_nan("") : (double)m);
+    return;
   }
-  return norm_join<NORM>(a0, a1);
+  float q[V / 2], s = 0.f;
+#pragma unroll
+  for (int e = 0; e < V / 2; ++e) {
+    q[e] = NORM == 0 ? fmaf(v[2 * e], v[2 * e], v[2 * e + 1] * v[2 * e + 1]) : fabsf(v[2 * e]) + fabsf(v[2 * e + 1]);
+    s += q[e];
+  }
+  if (s < 1e37f && (NORM == 1 || s > 1e-28f)) {
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) (e & 1 ? *a1 : *a0) += (double)q[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) *a0 = norm_acc<NORM>(*a0, v[e]);
+  }
 }
 
-template <int NORM>
+constexpr int DEEP = 8;                               // loads of at most 16 bytes that a thread has in flight
+
+// The `n` elements of a chunk by the workgroup's 256 threads: f(index, values) for whole vectors of V, one(index, value) for
+// the few elements behind the last one
+template <int V, bool STREAM, typename T, typename F, typename G>
+__device__ __forceinline__ void for_vectors(const T* p, int n, F f, G one) {
+  constexpr int TURN = DEEP * 256 * V;
+  typedef typename Vec<T, V>::type vec;
+  const int whole = n & ~(V - 1);
+  int base = 0;
+  for (; base + TURN <= whole; base += TURN) {
+    const int i0 = base + (int)threadIdx.x * V;
+    vec r[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      const TREBI_GLOBAL vec* q = (const TREBI_GLOBAL vec*)(p + i0 + u * 256 * V);
+      r[u] = STREAM ? __builtin_nontemporal_load(q) : *q;
+    }
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = up(r[u][e]);
+      f(i0 + u * 256 * V, v);
+    }
+  }
+  if (base < whole) {
+    const int i0 = base + (int)threadIdx.x * V;
+    vec r[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u)
+      if (i0 + u * 256 * V < whole) r[u] = *(const TREBI_GLOBAL vec*)(p + i0 + u * 256 * V);
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u)
+      if (i0 + u * 256 * V < whole) {
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = up(r[u][e]);
+        f(i0 + u * 256 * V, v);
+      }
+  }
+  if (whole + (int)threadIdx.x < n) one(whole + (int)threadIdx.x, load_one(p + whole + threadIdx.x));
+}
+
+template <int NORM, bool STREAM>
 __global__ __launch_bounds__(256) void grad_partial_kernel(GradP p) {
   __shared__ double lds[4];
-  double a = 0;
+  double a0 = 0, a1 = 0;
+  auto one = [&](int, float v) { a0 = norm_acc<NORM>(a0, v); };
   for (int c = blockIdx.x; c < p.n_chunks; c += gridDim.x) {
-    const GradChunk ch = p.chunks[c];
-    const GradTensor t = p.tensors[ch.tensor];
-    double v;
-    if (t.dtype == 0) v = chunk_norm<NORM>((const float*)t.p + ch.off, ch.len);
-    else if (t.dtype == 1) v = chunk_norm<NORM>((const bf16_t*)t.p + ch.off, ch.len);
-    else v = chunk_norm<NORM>((const f16_t*)t.p + ch.off, ch.len);
-    a = norm_join<NORM>(a, v);
+    const GradChunk t = uniform_load(p.chunks + c);
+    if (t.dtype == 0) for_vectors<4, STREAM>((const float*)t.p, t.len, [&](int, const float* v) { join_vec<NORM, 4>(v, &a0, &a1); }, one);
+    else if (t.dtype == 1) for_vectors<8, STREAM>((const bf16_t*)t.p, t.len, [&](int, const float* v) { join_vec<NORM, 8>(v, &a0, &a1); }, one);
+    else for_vectors<8, STREAM>((const f16_t*)t.p, t.len, [&](int, const float* v) { join_vec<NORM, 8>(v, &a0, &a1); }, one);
   }
-  a = block_join<NORM, 256>(a, lds);
+  const double a = block_join<NORM, 256>(norm_join<NORM>(a0, a1), lds);
   if (threadIdx.x == 0) p.part[blockIdx.x] = a;
 }
 
 // The norm from the partials, the same in every workgroup that asks.
+template <int NT>
 __device__ __forceinline__ float grad_total(const GradP& p, double* lds, float* coef) {
   double a = 0;
   if (p.norm_type == 2) {
-    for (int i = threadIdx.x; i < p.n_part; i += 256) a = norm_join<2>(a, p.part[i]);
-    a = block_join<2, 256>(a, lds);
+    for (int i = threadIdx.x; i < p.n_blocks; i += NT) a = norm_join<2>(a, p.part[i]);
+    a = block_join<2, NT>(a, lds);
   } else {
-    for (int i = threadIdx.x; i < p.n_part; i += 256) a += p.part[i];
-    a = block_join<0, 256>(a, lds);
+    for (int i = threadIdx.x; i < p.n_blocks; i += NT) a += p.part[i];
+    a = block_join<0, NT>(a, lds);
     if (p.norm_type == 0) a = sqrt(a);
   }
   const double n = a * (double)p.grad_scale;
@@ -101,82 +144,78 @@ __device__ __forceinline__ float grad_total(const GradP& p, double* lds, float* 
   return (float)n;
 }
 
-__global__ __launch_bounds__(256) void grad_finish_kernel(GradP p, float* coef_out) {
-  __shared__ double lds[4];
+__global__ __launch_bounds__(1024) void grad_finish_kernel(GradP p, float* coef_out) {
+  __shared__ double lds[16];
   float coef;
-  const float n = grad_total(p, lds, &coef);
+  const float n = grad_total<1024>(p, lds, &coef);
   if (threadIdx.x == 0) {
     if (p.norm_out) *p.norm_out = n;
     if (coef_out) *coef_out = coef;
   }
 }
 
-template <typename T, typename O>
-__device__ __forceinline__ void chunk_scale(const T* p, O* out, int len, float c) {
-  constexpr int V = 16 / sizeof(T);
-  int i = threadIdx.x * V;
-  for (; i + 3 * 256 * V + V <= len; i += 4 * 256 * V) {
-    float v[4][V];
+template <int V, bool STREAM, typename O>
+__device__ __forceinline__ void put_vec(O* p, const float* v) {
+  typedef typename Vec<O, V>::type vec;
+  vec r;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load_vec<V>(p + i + u * 256 * V, v[u]);
+  for (int e = 0; e < V; ++e) r[e] = down<O>(v[e]);
+  if (STREAM) __builtin_nontemporal_store(r, (TREBI_GLOBAL vec*)p);
+  else *(TREBI_GLOBAL vec*)p = r;
+}
+template <bool STREAM, typename T, typename O>
+__device__ __forceinline__ void scale_chunk(const T* p, O* out, int n, float c) {
+  constexpr int V = 16 / (int)sizeof(O);               // whole 16-byte stores, neighbouring lanes' next to each other
+  for_vectors<V, false>(p, n, [&](int i, float* v) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[u][e] *= c;
-      store_vec<V>(out + i + u * 256 * V, v[u]);
-    }
-  }
-  for (; i < len; i += 256 * V) {
-    if (i + V <= len) {
-      float v[V];
-      load_vec<V>(p + i, v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[e] *= c;
-      store_vec<V>(out + i, v);
-    } else {
-      for (int e = i; e < len; ++e) store_one(out + e, load_one(p + e) * c);
-    }
-  }
+    for (int e = 0; e < V; ++e) v[e] *= c;
+    put_vec<V, STREAM>(out + i, v);
+  }, [&](int i, float v) { store_one(out + i, v * c); });
 }
 
+// The chunks are walked backwards: what the norm's kernel read last is what the cache still holds.
+template <bool STREAM>
 __global__ __launch_bounds__(256) void grad_scale_kernel(GradP p) {
   __shared__ double lds[4];
+  GradChunk t = uniform_load(p.chunks + (p.n_chunks > 0 ? p.n_chunks - 1 - (int)blockIdx.x : 0));
   float c;
-  const float n = grad_total(p, lds, &c);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && p.norm_out) *p.norm_out = n;
+  const float norm = grad_total<256>(p, lds, &c);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.norm_out) *p.norm_out = norm;
   if (!p.out && c == 1.f) return;                     // in place and within the norm: nothing would change
-  for (int k = blockIdx.x; k < p.n_chunks; k += gridDim.x) {
-    const GradChunk ch = p.chunks[k];
-    const GradTensor t = p.tensors[ch.tensor];
-    float* o = p.out ? p.out + t.out_off + ch.off : nullptr;
-    if (t.dtype == 0) {
-      const float* g = (const float*)t.p + ch.off;
-      chunk_scale(g, o ? o : (float*)g, ch.len, c);
-    } else if (t.dtype == 1) {
-      const bf16_t* g = (const bf16_t*)t.p + ch.off;
-      if (o) chunk_scale(g, o, ch.len, c);
-      else chunk_scale(g, (bf16_t*)g, ch.len, c);
+  for (int q = blockIdx.x; q < p.n_chunks; q += gridDim.x) {
+    if (q > (int)blockIdx.x) t = uniform_load(p.chunks + p.n_chunks - 1 - q);
+    float* o = p.out ? p.out + t.out_off : nullptr;
+    if (t.dtype == 0) scale_chunk<STREAM>((const float*)t.p, o ? o : (float*)t.p, t.len, c);
+    else if (t.dtype == 1) {
+      if (o) scale_chunk<STREAM>((const bf16_t*)t.p, o, t.len, c);
+      else scale_chunk<STREAM>((const bf16_t*)t.p, (bf16_t*)t.p, t.len, c);
     } else {
-      const f16_t* g = (const f16_t*)t.p + ch.off;
-      if (o) chunk_scale(g, o, ch.len, c);
-      else chunk_scale(g, (f16_t*)g, ch.len, c);
+      if (o) scale_chunk<STREAM>((const f16_t*)t.p, o, t.len, c);
+      else scale_chunk<STREAM>((const f16_t*)t.p, (f16_t*)t.p, t.len, c);
     }
   }
 }
 
 hipError_t launch_grad_partials(const GradP& p, hipStream_t st) {
-  const dim3 g(p.n_part), b(256);
-  if (p.norm_type == 0) hipLaunchKernelGGL(grad_partial_kernel<0>, g, b, 0, st, p);
-  else if (p.norm_type == 1) hipLaunchKernelGGL(grad_partial_kernel<1>, g, b, 0, st, p);
-  else hipLaunchKernelGGL(grad_partial_kernel<2>, g, b, 0, st, p);
+  const dim3 g(p.n_blocks), b(256);
+#define GO(N)                                                                                  \
+  do {                                                                                         \
+    if (p.stream_loads) hipLaunchKernelGGL((grad_partial_kernel<N, true>), g, b, 0, st, p);    \
+    else hipLaunchKernelGGL((grad_partial_kernel<N, false>), g, b, 0, st, p);                  \
+  } while (0)
+  if (p.norm_type == 0) GO(0);
+  else if (p.norm_type == 1) GO(1);
+  else GO(2);
+#undef GO
   return hipGetLastError();
 }
 hipError_t launch_grad_finish(const GradP& p, float* coef_out, hipStream_t st) {
-  hipLaunchKernelGGL(grad_finish_kernel, dim3(1), dim3(256), 0, st, p, coef_out);
+  hipLaunchKernelGGL(grad_finish_kernel, dim3(1), dim3(1024), 0, st, p, coef_out);
   return hipGetLastError();
 }
 hipError_t launch_grad_scale(const GradP& p, hipStream_t st) {
-  hipLaunchKernelGGL(grad_scale_kernel, dim3(p.n_part), dim3(256), 0, st, p);
+  if (p.stream_stores) hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(p.n_blocks), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(p.n_blocks), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 

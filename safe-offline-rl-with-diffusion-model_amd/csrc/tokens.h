@@ -2,6 +2,7 @@
 // alignment (gfx950 takes vector accesses at element alignment), and block sums in a fixed order.
 #pragma once
 #include "device_util.h"
+#include "finetune.h"
 
 namespace trebi {
 
@@ -63,12 +64,64 @@ __device__ __forceinline__ void store_vec(T* p, const float* v) {
   }
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
+// N consecutive elements as they lie in memory: loaded first, widened when they are needed, so that the loads of a turn are
+// all on their way before the first of them is waited for.
+template <typename T, int N> struct Pack {
+  static constexpr int W = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
+  typename Vec<T, W>::type r[N / W];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+    for (int k = 0; k < N / W; ++k) r[k] = *(const TREBI_GLOBAL typename Vec<T, W>::type*)(p + k * W);
+  }
+  __device__ __forceinline__ float at(int e) const { return up(r[e / W][e % W]); }
+};
+
+// Loads through the scalar cache, at an index that is the same in every lane of the wave and from memory that nothing
+// writes while the kernel runs.  They are counted apart from the vector loads, which return in order: a look-up by vector
+// loads would wait for all the data asked for before it.
+template <typename T>
+__device__ __forceinline__ T uniform_load(const T* p) {
+  if constexpr (sizeof(T) <= 8) {
+    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+  } else {                                             // a struct of 8-byte words
+    union { T t; long long w[sizeof(T) / 8]; } c;
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T) / 8; ++k) c.w[k] = ((const __attribute__((address_space(4))) long long*)(uintptr_t)p)[k];
+    return c.t;
+  }
 }
-// Sum of K values over a workgroup of NT threads, in every thread; lds: [NT / 64][K].  The order is fixed.
+__device__ __forceinline__ long long uniform(long long v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)v);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)((unsigned long long)v >> 32));
+  return (long long)(((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  union { double d; int i[2]; } c, r;
+  c.d = v;
+  r.i[0] = __builtin_amdgcn_update_dpp(0, c.i[0], CTRL, 0xf, 0xf, false);
+  r.i[1] = __builtin_amdgcn_update_dpp(0, c.i[1], CTRL, 0xf, 0xf, false);
+  return r.d;
+}
+__device__ __forceinline__ double lane_d(double v, int lane) {
+  union { double d; int i[2]; } c, r;
+  c.d = v;
+  r.i[0] = __builtin_amdgcn_readlane(c.i[0], lane);
+  r.i[1] = __builtin_amdgcn_readlane(c.i[1], lane);
+  return r.d;
+}
+// Sum over the wave's 64 lanes (all of them active), in every lane; exchanges inside the registers, in a fixed order
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp_d<0xB1>(v);      // quad_perm [1,0,3,2]
+  v += dpp_d<0x4E>(v);      // quad_perm [2,3,0,1]
+  v += dpp_d<0x141>(v);     // row_half_mirror
+  v += dpp_d<0x140>(v);     // row_mirror
+  return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
+}
+// Sum of K values over a workgroup of NT threads, in a fixed order; lds: [NT / 64 + 1][K].  In every thread up to 256
+// threads, in thread 0 of a larger workgroup.
 template <int K, int NT>
 __device__ __forceinline__ void block_sum(double* v, double* lds) {
   __syncthreads();
@@ -78,12 +131,38 @@ __device__ __forceinline__ void block_sum(double* v, double* lds) {
 #pragma unroll
     for (int k = 0; k < K; ++k) lds[(threadIdx.x >> 6) * K + k] = v[k];
   __syncthreads();
+  if (NT <= 256) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    double a = 0;
+    for (int k = 0; k < K; ++k) {
+      double a = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) a += lds[w * K + k];
-    v[k] = a;
+      for (int w = 0; w < NT / 64; ++w) a += lds[w * K + k];
+      v[k] = a;
+    }
+  } else {
+    if (threadIdx.x < K) {
+      double a = 0;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) a += lds[w * K + threadIdx.x];
+      lds[(NT / 64) * K + threadIdx.x] = a;            // the first wave's own: no barrier
+    }
+    if (threadIdx.x == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = lds[(NT / 64) * K + k];
+  }
+}
+
+// Tokens [*s, *e) of row r, as columns (padded) or flat positions (packed); offsets that leave the buffer are cut.
+__device__ __forceinline__ void row_bounds(const TokenP& t, long long r, long long* s, long long* e) {
+  if (t.packed) {
+    long long a = t.cu[r], b = t.cu[r + 1];
+    a = a < 0 ? 0 : (a > t.n ? t.n : a);
+    *s = a;
+    *e = b < a ? a : (b > t.n ? t.n : b);
+  } else {
+    *s = 0;
+    long long b = t.lengths ? (long long)t.lengths[r] : t.len;
+    *e = b < 0 ? 0 : (b > t.len ? t.len : b);
   }
 }
 

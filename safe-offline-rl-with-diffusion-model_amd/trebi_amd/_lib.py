@@ -51,7 +51,7 @@ class LayerInfo(C.Structure):
 
 
 class GradSet(C.Structure):
-    _fields_ = [('n_tensors', C.c_int), ('n_chunks', C.c_int), ('total', C.c_int64)]
+    _fields_ = [('n_tensors', C.c_int), ('n_chunks', C.c_int), ('total', C.c_int64), ('bytes', C.c_int64)]
 
 
 class TokenDesc(C.Structure):

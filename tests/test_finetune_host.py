@@ -128,25 +128,24 @@ def fill(ptrs, numels, dtypes, table=None, short=0):
     return rc, s, buf
 
 
-def test_gradient_set_table_covers_every_element_once():
+@pytest.mark.parametrize('numels', [[0, 1, 7, 4096, 4097, 100000, 0, 33, 12289], [0], [1], [5] * 700, [20000000, 0, 3], [0] * 9,
+                                    [3584, 3585, 3583, 512, 0, 4096]])
+def test_gradient_set_table_covers_every_element_once(numels):
     rng = np.random.default_rng(3)
-    numels = [0, 1, 7, 4096, 4097, 100000, 0, 33, 12289]
     starts, at = [], 1 << 20
     for n in numels:
         starts.append(at)
         at += 4 * n + 4 * int(rng.integers(0, 5))
     rc, s, buf = fill(starts, numels, [0] * len(numels))
-    assert rc == 0 and s.n_tensors == len(numels) and s.total == sum(numels)
-    raw = buf.view(np.uint8)
-    tens = raw[:32 * len(numels)].view(np.dtype([('p', '<u8'), ('n', '<i8'), ('out', '<i8'), ('dtype', '<i4'), ('pad', '<i4')]))
-    assert [int(t['p']) for t in tens if t['n']] == [p for p, n in zip(starts, numels) if n]
-    assert list(tens['out']) == list(np.cumsum([0] + numels[:-1]))
-    base = (32 * len(numels) + 255) // 256 * 256
-    ch = raw[base:base + 16 * s.n_chunks].view(np.dtype([('off', '<i8'), ('tensor', '<i4'), ('len', '<i4')]))
+    assert rc == 0 and s.n_tensors == len(numels) and s.total == sum(numels) and s.bytes == 4 * s.total
+    ch = buf.view(np.uint8)[:24 * s.n_chunks].view(np.dtype([('p', '<u8'), ('out', '<i8'), ('len', '<i4'), ('dtype', '<i4')]))
     seen = [np.zeros(n, int) for n in numels]
+    first = np.cumsum([0] + numels)
     for c in ch:
-        assert c['len'] > 0
-        seen[c['tensor']][c['off']:c['off'] + c['len']] += 1
+        i = int(np.searchsorted(first, c['out'], side='right')) - 1        # the tensor (not empty) that the chunk's output lies in
+        off = int(c['out']) - int(first[i])
+        assert c['len'] > 0 and c['dtype'] == 0 and int(c['p']) == starts[i] + 4 * off and off + c['len'] <= numels[i]
+        seen[i][off:off + c['len']] += 1
     assert all((v == 1).all() for v in seen)
 
 
