@@ -6,6 +6,8 @@ raised.  PyTorch only supplies device memory and the current stream.
 import ctypes as C
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('TREBI_LIB') or os.path.join(_HERE, 'libtrebi_hip.so')   # TREBI_LIB: A/B builds on one box (diagnostics)
 
@@ -142,18 +144,17 @@ SIGNATURES = {
     'trebi_trainer_step': (C.c_int, [_VP, C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int, C.c_float,
                                      _VP]),
     'trebi_grad_set_bytes': (C.c_size_t, [C.c_int, c_i64_p]),
-    'trebi_grad_set_fill': (C.c_int, [C.c_int, C.POINTER(_VP), c_i64_p, C.POINTER(C.c_int), _VP, C.c_size_t,
-                                      C.POINTER(GradSet)]),
-    'trebi_grad_workspace_bytes': (C.c_size_t, [C.POINTER(GradSet)]),
-    'trebi_grad_norm': (C.c_int, [_VP, C.POINTER(GradSet), _VP, C.c_int, C.c_float, _VP, _VP, C.c_size_t, _VP]),
-    'trebi_grad_clip': (C.c_int, [_VP, C.POINTER(GradSet), _VP, C.c_int, C.c_float, C.c_float, _VP, _VP, _VP, C.c_size_t,
+    'trebi_grad_set_fill': (C.c_int, [C.c_int, C.POINTER(_VP), c_i64_p, C.POINTER(C.c_int), _VP, C.c_size_t, _VP]),
+    'trebi_grad_workspace_bytes': (C.c_size_t, [_VP]),
+    'trebi_grad_norm': (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_float, _VP, _VP, C.c_size_t, _VP]),
+    'trebi_grad_clip': (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_float, C.c_float, _VP, _VP, _VP, C.c_size_t,
                                   _VP]),
-    'trebi_policy_loss_workspace_bytes': (C.c_size_t, [C.POINTER(TokenDesc)]),
-    'trebi_policy_loss': (C.c_int, [_VP, C.POINTER(TokenDesc), C.POINTER(PolicyLossDesc), _VP, C.c_size_t, _VP]),
-    'trebi_preference_loss_workspace_bytes': (C.c_size_t, [C.POINTER(TokenDesc)]),
-    'trebi_preference_loss': (C.c_int, [_VP, C.POINTER(TokenDesc), C.POINTER(PreferenceLossDesc), _VP, C.c_size_t, _VP]),
-    'trebi_transition_logp': (C.c_int, [_VP, C.POINTER(TransitionDesc), _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP]),
-    'trebi_transition_logp_grad': (C.c_int, [_VP, C.POINTER(TransitionDesc), _VP, _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP]),
+    'trebi_policy_loss_workspace_bytes': (C.c_size_t, [_VP]),
+    'trebi_policy_loss': (C.c_int, [_VP, _VP, _VP, _VP, C.c_size_t, _VP]),
+    'trebi_preference_loss_workspace_bytes': (C.c_size_t, [_VP]),
+    'trebi_preference_loss': (C.c_int, [_VP, _VP, _VP, _VP, C.c_size_t, _VP]),
+    'trebi_transition_logp': (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP]),
+    'trebi_transition_logp_grad': (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, C.c_int64, _VP, _VP]),
 }
 
 _lib = None
@@ -180,6 +181,12 @@ def check(rc):
     if rc != 0:
         msg = lib().trebi_last_error()
         raise RuntimeError(f'trebi_hip error {rc}: {msg.decode() if msg else "?"}')
+
+
+def stream(device):
+    """The raw current stream of a CUDA device, as an int (what torch.cuda.current_stream(device).cuda_stream is, without
+    the Stream object, which costs a call of a few microseconds a good part of its time)."""
+    return torch._C._cuda_getCurrentRawStream(device.index or 0)
 
 
 _ctx = {}

@@ -63,7 +63,7 @@ class GradClipper:
     def _buffers(self):
         """A workspace of this call's own (two calls may run at once), the norm, the stream."""
         ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
-        return ws, torch.empty((), device=self.device), torch.cuda.current_stream(self.device).cuda_stream
+        return ws, torch.empty((), device=self.device), _lib.stream(self.device)
 
     def norm(self, grad_scale=1.0):
         """grad_scale * the norm, a device scalar."""

@@ -14,6 +14,7 @@ What stands at tokens that do not count is never used; their gradient is 0.  Inp
 type for all log-probabilities); advantages and weights float32.
 """
 import ctypes as C
+import struct
 from collections import namedtuple
 
 import torch
@@ -29,8 +30,14 @@ _REDUCTIONS = {'token': 0, 'sequence': 1}
 _KINDS = {'sigmoid': 0, 'hinge': 1, 'ipo': 2}
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# The library's descriptors (include/trebi_hip.h), packed: a ctypes Structure of this many fields takes longer to fill than a
+# small call runs on the GPU
+_TOKENS = struct.Struct('@qqiPPPqq')
+_POLICY = struct.Struct('@iPPPqqqqqqPqqPPffffiidf4x')
+_PREFERENCE = struct.Struct('@iPPqqqqPPPPPfffiidf4x')
+_TRANSITION = struct.Struct('@7i4iqqqPPPPP')
+assert [v.size for v in (_TOKENS, _POLICY, _PREFERENCE, _TRANSITION)] == [
+    C.sizeof(v) for v in (_lib.TokenDesc, _lib.PolicyLossDesc, _lib.PreferenceLossDesc, _lib.TransitionDesc)]
 
 
 def _check_logp(logp):
@@ -80,17 +87,15 @@ def _token_desc(logp, mask, lengths, cu_seqlens):
             mask = mask.contiguous()
         keep += [cu, mask]
         rows = cu.numel() - 1
-        d = _lib.TokenDesc(rows, logp.numel(), 1, None, cu.data_ptr(), None if mask is None else mask.data_ptr(), 0, 1)
+        d = _TOKENS.pack(rows, logp.numel(), 1, 0, cu.data_ptr(), 0 if mask is None else mask.data_ptr(), 0, 1)
         return d, rows, keep
     rows, length = logp.shape
-    at = None
-    if lengths is not None:
-        at = _ints('lengths', lengths, rows, dev)
-    keep += [at, mask]
+    if lengths is None and mask is None:
+        return _TOKENS.pack(rows, length, 0, 0, 0, 0, 0, 1), rows, None
+    at = None if lengths is None else _ints('lengths', lengths, rows, dev)
     ms = (0, 1) if mask is None else mask.stride()
-    d = _lib.TokenDesc(rows, length, 0, None if at is None else at.data_ptr(), None,
-                       None if mask is None else mask.data_ptr(), ms[0], ms[1])
-    return d, rows, keep
+    d = _TOKENS.pack(rows, length, 0, 0 if at is None else at.data_ptr(), 0, 0 if mask is None else mask.data_ptr(), *ms)
+    return d, rows, (at, mask)
 
 
 def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=None, clip=0.2,
@@ -152,14 +157,17 @@ def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, le
         return PolicyLoss(z[0], None if grad is None else grad.zero_().reshape(shape), *z[1:])
     stats = torch.empty(5, device=dev)
     lib = _lib.lib()
-    ws = torch.empty(lib.trebi_policy_loss_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=dev)
-    q = _lib.PolicyLossDesc(
-        _DTYPES[logp.dtype], logp.data_ptr(), None if logp_old is None else logp_old.data_ptr(),
-        None if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1], *strides[2], advantages.data_ptr(),
-        *adv_stride, None if grad is None else grad.data_ptr(), stats.data_ptr(), clip, clip if clip_high is None else clip_high,
+    ws_bytes = lib.trebi_policy_loss_workspace_bytes(d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    q = _POLICY.pack(
+        _DTYPES[logp.dtype], logp.data_ptr(), 0 if logp_old is None else logp_old.data_ptr(),
+        0 if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1], *strides[2], advantages.data_ptr(),
+        *adv_stride, 0 if grad is None else grad.data_ptr(), stats.data_ptr(), clip, clip if clip_high is None else clip_high,
         0.0 if dual_clip is None else dual_clip, kl_coef, _KL[kl], _REDUCTIONS[reduction] if denominator is None else 2,
         0.0 if denominator is None else denominator, grad_scale)
-    _lib.check(lib.trebi_policy_loss(_lib.ctx(dev.index or 0), C.byref(d), C.byref(q), ws.data_ptr(), ws.numel(), _stream(dev)))
+    rc = lib.trebi_policy_loss(_lib.ctx(dev.index or 0), d, q, ws.data_ptr(), ws_bytes, _lib.stream(dev))
+    if rc:
+        _lib.check(rc)
     loss, policy, klv, cut, ratio = stats.unbind()
     return PolicyLoss(loss, grad if grad is None or grad.shape == shape else grad.reshape(shape), policy, klv, cut, ratio)
 
@@ -213,16 +221,18 @@ def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=
         e = torch.empty(0, device=dev)
         return PreferenceLoss(z[0], None if grad is None else grad.zero_().reshape(shape), e, e.clone(), z[1], z[2])
     out = torch.empty(2 * P + 3, device=dev)
-    chosen, rejected, stats = out[:P], out[P:2 * P], out[2 * P:]
     lib = _lib.lib()
-    ws = torch.empty(lib.trebi_preference_loss_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=dev)
+    ws_bytes = lib.trebi_preference_loss_workspace_bytes(d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     at = out.data_ptr()
-    q = _lib.PreferenceLossDesc(
-        _DTYPES[logp.dtype], logp.data_ptr() or None, None if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1],
-        None if weights is None else weights.data_ptr(), None if grad is None else grad.data_ptr() or None, at, at + 4 * P,
-        at + 8 * P, beta, label_smoothing, margin, _KINDS[kind], int(bool(average)), 0.0 if denominator is None else denominator,
-        grad_scale)
-    _lib.check(lib.trebi_preference_loss(_lib.ctx(dev.index or 0), C.byref(d), C.byref(q), ws.data_ptr(), ws.numel(), _stream(dev)))
+    q = _PREFERENCE.pack(
+        _DTYPES[logp.dtype], logp.data_ptr(), 0 if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1],
+        0 if weights is None else weights.data_ptr(), 0 if grad is None else grad.data_ptr(), at, at + 4 * P, at + 8 * P, beta,
+        label_smoothing, margin, _KINDS[kind], int(bool(average)), 0.0 if denominator is None else denominator, grad_scale)
+    rc = lib.trebi_preference_loss(_lib.ctx(dev.index or 0), d, q, ws.data_ptr(), ws_bytes, _lib.stream(dev))
+    if rc:
+        _lib.check(rc)
+    chosen, rejected, stats = out.split((P, P, 3))
     loss, acc, mz = stats.unbind()
     return PreferenceLoss(loss, grad if grad is None or grad.shape == shape else grad.reshape(shape), chosen, rejected, acc, mz)
 
@@ -232,45 +242,50 @@ def _rows(name, v, shape, device):
     """float32 [B, H, D] whose candidates are contiguous (a slice of a chain keeps its stride), copied otherwise."""
     if v.shape != shape or v.device != device:
         raise ValueError(f'{name} is {tuple(v.shape)} on {v.device}, expected {tuple(shape)} on {device}')
-    if v.dtype != torch.float32:
+    if v.dtype is not torch.float32:
         raise TypeError(f'{name} must be float32, got {v.dtype}')
-    if v.stride(2) != 1 and shape[2] > 1 or v.stride(1) != shape[2] and shape[1] > 1:
+    s = v.stride()
+    if s[2] != 1 and shape[2] > 1 or s[1] != shape[2] and shape[1] > 1:
         v = v.contiguous()
-    return v, v.stride(0)
+        s = v.stride()
+    return v, s[0]
+
+
+_TABLES = ('posterior_log_variance_clipped', 'posterior_mean_coef1', 'posterior_mean_coef2')
+_NOISE_TABLES = ('sqrt_recip_alphas_cumprod', 'sqrt_recipm1_alphas_cumprod')
 
 
 def _transition(model, pred, x, x_prev, t, cond_keys):
-    dev = pred.device
+    dev, shape, T = pred.device, pred.shape, model.n_timesteps
     if dev.type != 'cuda':
         raise RuntimeError('trebi_amd computes transition log-probabilities on an MI355X only; there is no CPU path')
-    if pred.dim() != 3 or pred.shape[2] != model.transition_dim:
-        raise ValueError(f'pred must be [batch, horizon, {model.transition_dim}], got {tuple(pred.shape)}')
-    B, H, D = pred.shape
-    pred, ps = _rows('pred', pred, pred.shape, dev)
-    x, xs = _rows('x', x, pred.shape, dev)
-    x_prev, qs = _rows('x_prev', x_prev, pred.shape, dev)
+    if len(shape) != 3 or shape[2] != model.transition_dim:
+        raise ValueError(f'pred must be [batch, horizon, {model.transition_dim}], got {tuple(shape)}')
+    B, H, D = shape
+    pred, ps = _rows('pred', pred, shape, dev)
+    x, xs = _rows('x', x, shape, dev)
+    x_prev, qs = _rows('x_prev', x_prev, shape, dev)
     if not torch.is_tensor(t):
         t = torch.as_tensor(t)
     if t.dim() == 0:
         t = t.expand(B)
     if t.shape != (B,) or t.is_floating_point():
         raise ValueError(f't must be [{B}] integers, got {t.dtype} {tuple(t.shape)}')
-    if not t.is_cuda and B and not (0 <= int(t.min()) and int(t.max()) < model.n_timesteps):
-        raise RuntimeError(f'timesteps must lie in [0, {model.n_timesteps})')
+    if not t.is_cuda and B and not (0 <= int(t.min()) and int(t.max()) < T):
+        raise RuntimeError(f'timesteps must lie in [0, {T})')
     t = t.to(dev, torch.int64).contiguous()
     keys = sorted(int(k) for k in cond_keys)
     if len(keys) > 4:
         raise RuntimeError('at most 4 conditioned timesteps are supported')
-    names = ['posterior_log_variance_clipped', 'posterior_mean_coef1', 'posterior_mean_coef2']
-    if model.predict_epsilon:
-        names += ['sqrt_recip_alphas_cumprod', 'sqrt_recipm1_alphas_cumprod']
-    tabs = [getattr(model, n) for n in names]
-    for n, tab in zip(names, tabs):
-        if tab.device != dev or tab.dtype != torch.float32 or tab.shape != (model.n_timesteps,) or not tab.is_contiguous():
-            raise RuntimeError(f'{n} must be a contiguous float32 [{model.n_timesteps}] on {dev}')
-    ptrs = [tab.data_ptr() for tab in tabs] + [None] * (5 - len(tabs))
-    d = _lib.TransitionDesc(H, D, model.action_dim, model.observation_dim, model.n_timesteps, int(bool(model.clip_denoised)),
-                            len(keys), (C.c_int * 4)(*keys), ps, xs, qs, *ptrs)
+    ptrs = []
+    for n in _TABLES + _NOISE_TABLES if model.predict_epsilon else _TABLES:
+        tab = getattr(model, n)
+        if tab.device != dev or tab.dtype is not torch.float32 or tab.shape != (T,) or not tab.is_contiguous():
+            raise RuntimeError(f'{n} must be a contiguous float32 [{T}] on {dev}')
+        ptrs.append(tab.data_ptr())
+    ptrs += [0] * (5 - len(ptrs))
+    d = _TRANSITION.pack(H, D, model.action_dim, model.observation_dim, T, 1 if model.clip_denoised else 0, len(keys),
+                         *keys, *[0] * (4 - len(keys)), ps, xs, qs, *ptrs)
     return d, pred, x, x_prev, t
 
 
@@ -281,24 +296,27 @@ def transition_log_prob(model, pred, x, x_prev, t, cond_keys=(0,)):
     transition at t = 0, which adds no noise, has log-probability 0.  x and x_prev may be slices of a returned chain.  (A CUDA
     t is not checked here: the kernels cut it to the tables.)"""
     d, pred, x, x_prev, t = _transition(model, pred, x, x_prev, t, cond_keys)
-    B = pred.shape[0]
-    logp = torch.empty(B, device=pred.device)
+    B, dev = pred.shape[0], pred.device
+    logp = torch.empty(B, device=dev)
     if B:
-        _lib.check(_lib.lib().trebi_transition_logp(_lib.ctx(pred.device.index or 0), C.byref(d), pred.data_ptr(), x.data_ptr(),
-                                                    x_prev.data_ptr(), t.data_ptr(), B, logp.data_ptr(), _stream(pred.device)))
+        rc = _lib.lib().trebi_transition_logp(_lib.ctx(dev.index or 0), d, pred.data_ptr(), x.data_ptr(), x_prev.data_ptr(),
+                                              t.data_ptr(), B, logp.data_ptr(), _lib.stream(dev))
+        if rc:
+            _lib.check(rc)
     return logp
 
 
 def transition_log_prob_grad(model, pred, x, x_prev, t, grad, cond_keys=(0,)):
     """grad[b] * d transition_log_prob[b] / d pred, [B, H, D]; `grad`: float32 [B], d loss / d log-probability."""
     d, pred, x, x_prev, t = _transition(model, pred, x, x_prev, t, cond_keys)
-    B = pred.shape[0]
-    if grad.shape != (B,) or grad.dtype != torch.float32 or grad.device != pred.device:
-        raise ValueError(f'grad must be float32 [{B}] on {pred.device}, got {grad.dtype} {tuple(grad.shape)} on {grad.device}')
+    B, dev = pred.shape[0], pred.device
+    if grad.shape != (B,) or grad.dtype is not torch.float32 or grad.device != dev:
+        raise ValueError(f'grad must be float32 [{B}] on {dev}, got {grad.dtype} {tuple(grad.shape)} on {grad.device}')
     grad = grad.contiguous()
-    out = torch.empty(pred.shape, device=pred.device)
+    out = torch.empty(pred.shape, device=dev)
     if B:
-        _lib.check(_lib.lib().trebi_transition_logp_grad(
-            _lib.ctx(pred.device.index or 0), C.byref(d), pred.data_ptr(), x.data_ptr(), x_prev.data_ptr(), t.data_ptr(),
-            grad.data_ptr(), B, out.data_ptr(), _stream(pred.device)))
+        rc = _lib.lib().trebi_transition_logp_grad(_lib.ctx(dev.index or 0), d, pred.data_ptr(), x.data_ptr(), x_prev.data_ptr(),
+                                                   t.data_ptr(), grad.data_ptr(), B, out.data_ptr(), _lib.stream(dev))
+        if rc:
+            _lib.check(rc)
     return out
