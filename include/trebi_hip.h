@@ -339,6 +339,20 @@ int trebi_trainer_set_bucket_event(trebi_trainer* tr, void* event);
 int trebi_trainer_step(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps,
                        int ema_mode, float ema_decay, void* stream);
 
+/* The same step with the gradient clipped to a global two-norm of max_norm first (see trebi_grad_clip; no counterpart in the
+ * reference): the factor is applied as Adam reads the gradient.  norm_out: dev [1], the norm before clipping, or null. */
+int trebi_trainer_step_clipped(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps,
+                               int ema_mode, float ema_decay, float max_norm, float* norm_out, void* stream);
+
+/* trebi_trainer_accumulate in two halves, for a loss of the caller's own (no counterpart in the reference):
+ *   pred = unet(x, t) with everything its backward reads kept in the trainer's workspace, then
+ *   grads += (d pred / d params)^T grad_pred.
+ * x, pred, grad_pred: dev [B, horizon, transition_dim], 16-byte aligned; x as the net is to see it (nothing is added or
+ * conditioned).  The backward must follow its forward on the same x, t and B, with no other call on this trainer between;
+ * it uses the forward up (a second backward is refused). */
+int trebi_trainer_forward(trebi_trainer* tr, const float* x, const int64_t* t, float* pred, int B, void* stream);
+int trebi_trainer_backward(trebi_trainer* tr, const float* x, const int64_t* t, const float* grad_pred, int B, void* stream);
+
 /* ---- fine-tuning ------------------------------------------------------------------
  * What follows the imitation of the training step above: policy-gradient and preference fine-tuning of the denoiser,
  * and the clipping that keeps such steps stable.  No counterpart in the reference.  These calls allocate nothing, keep

@@ -243,7 +243,7 @@ constexpr int LOSS_BLOCKS = 512;
 hipError_t launch_loss(const StepP& s, const float* pred, const float* targ, const float* w, int l1, float inv_count,
                        float inv_a0, float gscale, float* dout, float* partial, float* loss_out, int B, hipStream_t st);
 hipError_t launch_adam_ema(float* p, float* g, float* m, float* v, float* ema, long n, float b1, float b2, float step_size,
-                           float inv_bc2_sqrt, float eps, int ema_mode, float ema_decay, hipStream_t st);
+                           float inv_bc2_sqrt, float eps, int ema_mode, float ema_decay, const float* gscale, hipStream_t st);
 hipError_t launch_time_embed_train(const float* w1, const float* b1, const float* w2, const float* b2, int dim, int T,
                                    float* e /*[T,dim]*/, float* a1 /*[T,4dim]*/, float* temb /*[T,dim]*/, hipStream_t st);
 struct TBJob { const float* G; const float* Wt; float* gW; float* gb; float* DT; int C; int pad; };

@@ -629,10 +629,12 @@ hipError_t launch_make_map(const float* coded, int* map, long n, hipStream_t st)
 // torch.optim.Adam (bias-corrected, eps added after the corrected sqrt) + the trainer's EMA copy + zero_grad
 //   ema_mode 0: leave, 1: ema = p (training.py:95-97), 2: ema = ema*decay + (1-decay)*p (training.py:32-35)
 // =====================================================================================================
+//   gscale: what every gradient is multiplied by first (the clipping factor), or null
 __global__ void adam_ema_kernel(float* p, float* g, float* m, float* v, float* ema, long n, float b1, float b2,
-                                float step_size, float inv_bc2_sqrt, float eps, int ema_mode, float decay) {
+                                float step_size, float inv_bc2_sqrt, float eps, int ema_mode, float decay, const float* gscale) {
+  const float gs = gscale ? *gscale : 1.f;
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
-    const float gi = g[i];
+    const float gi = gscale ? g[i] * gs : g[i];
     const float mi = b1 * m[i] + (1.f - b1) * gi;
     const float vi = b2 * v[i] + (1.f - b2) * gi * gi;
     m[i] = mi;
@@ -646,10 +648,10 @@ __global__ void adam_ema_kernel(float* p, float* g, float* m, float* v, float* e
   }
 }
 hipError_t launch_adam_ema(float* p, float* g, float* m, float* v, float* ema, long n, float b1, float b2, float step_size,
-                           float inv_bc2_sqrt, float eps, int ema_mode, float ema_decay, hipStream_t st) {
+                           float inv_bc2_sqrt, float eps, int ema_mode, float ema_decay, const float* gscale, hipStream_t st) {
   int blocks = (int)std::min<long>((n + 255) / 256, 8192);
   hipLaunchKernelGGL(adam_ema_kernel, dim3(blocks), dim3(256), 0, st, p, g, m, v, ema, n, b1, b2, step_size, inv_bc2_sqrt,
-                     eps, ema_mode, ema_decay);
+                     eps, ema_mode, ema_decay, gscale);
   return hipGetLastError();
 }
 

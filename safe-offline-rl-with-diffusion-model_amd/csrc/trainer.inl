@@ -260,8 +260,15 @@ struct trebi_trainer {
   hipEvent_t bucket_event = nullptr;   // caller-owned: recorded when grads[split_off, total) are final
   float *params = nullptr, *grads = nullptr, *m = nullptr, *v = nullptr, *ema = nullptr;
   bool bound = false;
+  const float* fwd_x = nullptr;     // what trebi_trainer_forward last ran on (its activations are in ws), null: nothing
+  const int64_t* fwd_t = nullptr;
+  int fwd_B = 0;
+  // clipping of the flat gradient inside the optimiser step: one chunk table, partial sums, the factor
+  void* grad_table = nullptr;
+  trebi_grad_set grad_set{};
   std::map<int, std::vector<Tile>> tiles_fwd, tiles_bwd;
   ~trebi_trainer() {
+    if (grad_table) (void)hipFree(grad_table);
     for (int* p : maps) (void)hipFree(p);
     if (arena) (void)hipFree(arena);
     if (dev_rjobs) (void)hipFree(dev_rjobs);
@@ -511,6 +518,19 @@ extern "C" int trebi_trainer_bind(trebi_trainer* tr, float* params, float* grads
   tr->n_tb = (int)tb.size();
   HIPCHK(hipMalloc((void**)&tr->dev_tbjobs, tb.size() * sizeof(TBJob)));
   HIPCHK(hipMemcpy(tr->dev_tbjobs, tb.data(), tb.size() * sizeof(TBJob), hipMemcpyHostToDevice));
+  {
+    const int64_t numel = tr->pi.total;
+    const int f32 = TREBI_F32;
+    const void* g = grads;
+    const size_t table = trebi_grad_set_bytes(1, &numel), ws = trebi_grad_workspace_bytes(&tr->grad_set);
+    std::vector<char> host(table);
+    if (int e = trebi_grad_set_fill(1, &g, &numel, &f32, host.data(), table, &tr->grad_set)) return e;
+    if (tr->grad_table) (void)hipFree(tr->grad_table);
+    tr->grad_table = nullptr;
+    HIPCHK(hipMalloc(&tr->grad_table, table + ws + 256));
+    HIPCHK(hipMemcpy(tr->grad_table, host.data(), table, hipMemcpyHostToDevice));
+  }
+  tr->fwd_x = nullptr;
   tr->bound = true;
   if (int e = trainer_repack(tr, 0)) return e;
   HIPCHK(hipDeviceSynchronize());
@@ -542,60 +562,43 @@ int launch_op(const Op& op, const Resolver& r, Tile tl, hipStream_t st) {
 }
 }  // namespace
 
-extern "C" int trebi_trainer_accumulate(trebi_trainer* tr, const float* x_start, const float* const* cond,
-                                        const int64_t* tsteps, const float* noise, int B, float grad_scale,
-                                        float* loss_out, void* stream) {
-  if (!tr || !x_start || !tsteps || !noise || !loss_out) return fail(TREBI_BAD_ARG, "null argument");
-  if (!tr->bound) return fail(TREBI_BAD_ARG, "trebi_trainer_bind has not been called");
-  if (B < 1 || B > tr->maxB) return fail(TREBI_BAD_SHAPE, "batch %d outside 1..%d (max_batch of trebi_trainer_create)", B, tr->maxB);
-  if (tr->d.n_cond > 0 && !cond) return fail(TREBI_BAD_ARG, "cond is null");
-  hipStream_t st = (hipStream_t)stream;
-  HIPCHK(hipSetDevice(tr->ctx->device));
+// Tiles of every conv launch for a batch size (resolved once).
+// (per batch size AND operand mode: the chooser prices the fp32-only K loops differently)
+static int trainer_tiles(trebi_trainer* tr, int B, const std::vector<Tile>** tf, const std::vector<Tile>** tb) {
   trebi_net* net = tr->net;
-  const trebi_train_desc& d = tr->d;
-  const int H = d.horizon, D = net->desc.transition_dim, T = d.n_timesteps, dim = net->desc.dim;
-  StepP sp{};
-  sp.H = H; sp.D = D; sp.act = d.action_dim; sp.obs = d.observation_dim; sp.T = T; sp.n_cond = d.n_cond;
-  for (int k = 0; k < d.n_cond; ++k) {
-    if (!cond[k]) return fail(TREBI_BAD_ARG, "cond[%d] is null", k);
-    if (d.cond_index[k] < 0 || d.cond_index[k] >= H) return fail(TREBI_BAD_SHAPE, "conditioned index outside the horizon");
-    sp.cond_index[k] = d.cond_index[k];
-    sp.cond[k] = cond[k];
-  }
-  // ---- tiles of every conv launch for this batch size (resolved once) ----
-  // (per batch size AND operand mode: the chooser prices the fp32-only K loops differently)
   const int tkey = B | (net->prec == 1 ? 1 << 30 : 0);
   auto itf = tr->tiles_fwd.find(tkey);
   if (itf == tr->tiles_fwd.end()) {
-    std::vector<Tile> tf(net->fwd.size()), tb(net->tops.size());
+    std::vector<Tile> f(net->fwd.size()), w(net->tops.size());
     try {
-      for (size_t i = 0; i < net->fwd.size(); ++i) tf[i] = choose_tile(net->fwd[i], B, 1, use_bf(net, net->fwd[i], B));
+      for (size_t i = 0; i < net->fwd.size(); ++i) f[i] = choose_tile(net->fwd[i], B, 1, use_bf(net, net->fwd[i], B));
       for (size_t i = 0; i < net->tops.size(); ++i)
-        if (net->tops[i].kind == 0) tb[i] = choose_tile(net->tops[i].conv, B, 1, use_bf(net, net->tops[i].conv, B));
+        if (net->tops[i].kind == 0) w[i] = choose_tile(net->tops[i].conv, B, 1, use_bf(net, net->tops[i].conv, B));
     } catch (const Unsupported& u) {
       return fail(TREBI_UNSUPPORTED_CONFIG, "%s", u.msg.c_str());
     }
-    tr->tiles_bwd[tkey] = tb;
-    itf = tr->tiles_fwd.emplace(tkey, tf).first;
+    tr->tiles_bwd[tkey] = w;
+    itf = tr->tiles_fwd.emplace(tkey, f).first;
   }
-  const std::vector<Tile>& tf = itf->second;
-  const std::vector<Tile>& tbw = tr->tiles_bwd[tkey];
+  *tf = &itf->second;
+  *tb = &tr->tiles_bwd[tkey];
+  return 0;
+}
 
+// The forward on x, keeping what the backward reads: pred = unet(x, t), [B, H, D].
+static int trainer_forward(trebi_trainer* tr, const Resolver& r, const std::vector<Tile>& tf, int B, hipStream_t st) {
+  trebi_net* net = tr->net;
   if (poison_on())
     if (int e = poison_ws(tr->ws, net->ws_floats(B), st)) return e;
-  // ---- q_sample + conditioning, forward, loss (diffusion.py:240-254) ----
-  HIPCHK(launch_qsample(sp, x_start, noise, (const long long*)tsteps, tr->sa, tr->sb, tr->xnoisy, B, st));
-  Binding b;
-  b.x = tr->xnoisy; b.ldx = D; b.out = tr->pred; b.ldo = D; b.grad = tr->dout; b.ldg = D;
-  b.t = (const long long*)tsteps; b.t_uniform = -1; b.ws = tr->ws;
-  Resolver r{net, net->offsets(B), b, B};
   for (size_t i = 0; i < net->fwd.size(); ++i)
     if (int e = launch_op(net->fwd[i], r, tf[i], st)) return e;
-  const float inv_count = 1.f / ((float)B * H * D), inv_a0 = d.action_dim > 0 ? 1.f / ((float)B * d.action_dim) : 0.f;
-  HIPCHK(launch_loss(sp, tr->pred, d.predict_epsilon ? noise : x_start, tr->lw, d.loss_l1, inv_count, inv_a0,
-                     grad_scale * inv_count, tr->dout, tr->lossp, loss_out, B, st));
+  return 0;
+}
 
-  // ---- backward ----
+// The backward of the forward that r was resolved for: grads += d loss / d params, given r's gradient of the output.
+static int trainer_backward(trebi_trainer* tr, const Resolver& r, const std::vector<Tile>& tbw, const int64_t* tsteps, int B, hipStream_t st) {
+  trebi_net* net = tr->net;
+  const int T = tr->d.n_timesteps, dim = net->desc.dim;
   // partial tables -> gradients and the per-block time Linears, per bucket: the tail bucket's parameters
   // (final_conv, up path, mid blocks) are final once tops[0..top_split) have run, the rest at the end.
   auto finish_bucket = [&](int which) -> int {
@@ -680,17 +683,114 @@ extern "C" int trebi_trainer_accumulate(trebi_trainer* tr, const float* x_start,
   return 0;
 }
 
-extern "C" int trebi_trainer_step(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps,
-                                  int ema_mode, float ema_decay, void* stream) {
+static Binding trainer_binding(trebi_trainer* tr, const float* x, const int64_t* tsteps, float* pred, float* dpred) {
+  const int D = tr->net->desc.transition_dim;
+  Binding b;
+  b.x = x; b.ldx = D; b.out = pred; b.ldo = D; b.grad = dpred; b.ldg = D;
+  b.t = (const long long*)tsteps; b.t_uniform = -1; b.ws = tr->ws;
+  return b;
+}
+
+extern "C" int trebi_trainer_accumulate(trebi_trainer* tr, const float* x_start, const float* const* cond,
+                                        const int64_t* tsteps, const float* noise, int B, float grad_scale,
+                                        float* loss_out, void* stream) {
+  if (!tr || !x_start || !tsteps || !noise || !loss_out) return fail(TREBI_BAD_ARG, "null argument");
+  if (!tr->bound) return fail(TREBI_BAD_ARG, "trebi_trainer_bind has not been called");
+  if (B < 1 || B > tr->maxB) return fail(TREBI_BAD_SHAPE, "batch %d outside 1..%d (max_batch of trebi_trainer_create)", B, tr->maxB);
+  if (tr->d.n_cond > 0 && !cond) return fail(TREBI_BAD_ARG, "cond is null");
+  hipStream_t st = (hipStream_t)stream;
+  HIPCHK(hipSetDevice(tr->ctx->device));
+  trebi_net* net = tr->net;
+  const trebi_train_desc& d = tr->d;
+  const int H = d.horizon, D = net->desc.transition_dim, T = d.n_timesteps;
+  StepP sp{};
+  sp.H = H; sp.D = D; sp.act = d.action_dim; sp.obs = d.observation_dim; sp.T = T; sp.n_cond = d.n_cond;
+  for (int k = 0; k < d.n_cond; ++k) {
+    if (!cond[k]) return fail(TREBI_BAD_ARG, "cond[%d] is null", k);
+    if (d.cond_index[k] < 0 || d.cond_index[k] >= H) return fail(TREBI_BAD_SHAPE, "conditioned index outside the horizon");
+    sp.cond_index[k] = d.cond_index[k];
+    sp.cond[k] = cond[k];
+  }
+  const std::vector<Tile>*tf, *tbw;
+  if (int e = trainer_tiles(tr, B, &tf, &tbw)) return e;
+  tr->fwd_x = nullptr;
+  // ---- q_sample + conditioning, forward, loss (diffusion.py:240-254), backward ----
+  HIPCHK(launch_qsample(sp, x_start, noise, (const long long*)tsteps, tr->sa, tr->sb, tr->xnoisy, B, st));
+  Resolver r{net, net->offsets(B), trainer_binding(tr, tr->xnoisy, tsteps, tr->pred, tr->dout), B};
+  if (int e = trainer_forward(tr, r, *tf, B, st)) return e;
+  const float inv_count = 1.f / ((float)B * H * D), inv_a0 = d.action_dim > 0 ? 1.f / ((float)B * d.action_dim) : 0.f;
+  HIPCHK(launch_loss(sp, tr->pred, d.predict_epsilon ? noise : x_start, tr->lw, d.loss_l1, inv_count, inv_a0,
+                     grad_scale * inv_count, tr->dout, tr->lossp, loss_out, B, st));
+  return trainer_backward(tr, r, *tbw, tsteps, B, st);
+}
+
+// ---- any other loss: forward, the caller's own gradient of the output, backward ----
+static int trainer_io(trebi_trainer* tr, const float* x, const int64_t* tsteps, const float* out, int B) {
+  if (!tr || !x || !tsteps || !out) return fail(TREBI_BAD_ARG, "null argument");
+  if (!tr->bound) return fail(TREBI_BAD_ARG, "trebi_trainer_bind has not been called");
+  if (B < 1 || B > tr->maxB) return fail(TREBI_BAD_SHAPE, "batch %d outside 1..%d (max_batch of trebi_trainer_create)", B, tr->maxB);
+  if (((uintptr_t)x | (uintptr_t)out) & 15) return fail(TREBI_BAD_ARG, "x and the output (gradient) must be 16-byte aligned");
+  return 0;
+}
+
+extern "C" int trebi_trainer_forward(trebi_trainer* tr, const float* x, const int64_t* tsteps, float* pred, int B, void* stream) {
+  if (int e = trainer_io(tr, x, tsteps, pred, B)) return e;
+  HIPCHK(hipSetDevice(tr->ctx->device));
+  const std::vector<Tile>*tf, *tbw;
+  if (int e = trainer_tiles(tr, B, &tf, &tbw)) return e;
+  Resolver r{tr->net, tr->net->offsets(B), trainer_binding(tr, x, tsteps, pred, nullptr), B};
+  tr->fwd_x = nullptr;
+  if (int e = trainer_forward(tr, r, *tf, B, (hipStream_t)stream)) return e;
+  tr->fwd_x = x; tr->fwd_t = tsteps; tr->fwd_B = B;
+  return 0;
+}
+
+extern "C" int trebi_trainer_backward(trebi_trainer* tr, const float* x, const int64_t* tsteps, const float* grad_pred, int B, void* stream) {
+  if (int e = trainer_io(tr, x, tsteps, grad_pred, B)) return e;
+  if (tr->fwd_x != x || tr->fwd_t != tsteps || tr->fwd_B != B)
+    return fail(TREBI_BAD_ARG, "the last call on this trainer was not trebi_trainer_forward on the same x, t and batch");
+  HIPCHK(hipSetDevice(tr->ctx->device));
+  const std::vector<Tile>*tf, *tbw;
+  if (int e = trainer_tiles(tr, B, &tf, &tbw)) return e;
+  Resolver r{tr->net, tr->net->offsets(B), trainer_binding(tr, x, tsteps, nullptr, const_cast<float*>(grad_pred)), B};
+  tr->fwd_x = nullptr;                             // the backward overwrites what the forward kept
+  return trainer_backward(tr, r, *tbw, tsteps, B, (hipStream_t)stream);
+}
+
+static int trainer_step(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps, int ema_mode,
+                        float ema_decay, bool clip, float max_norm, float* norm_out, hipStream_t st) {
   if (!tr || !tr->bound) return fail(TREBI_BAD_ARG, "trainer is null or not bound");
   if (!tr->m || !tr->v) return fail(TREBI_BAD_ARG, "no Adam moment buffers were bound");
   if (adam_step < 1) return fail(TREBI_BAD_ARG, "adam_step counts from 1");
   if (ema_mode < 0 || ema_mode > 2 || (ema_mode && !tr->ema)) return fail(TREBI_BAD_ARG, "bad ema_mode / no EMA buffer bound");
-  hipStream_t st = (hipStream_t)stream;
+  if (clip && !(max_norm >= 0.f)) return fail(TREBI_BAD_ARG, "max_norm must not be negative");
   HIPCHK(hipSetDevice(tr->ctx->device));
+  tr->fwd_x = nullptr;
+  const float* coef = nullptr;
+  if (clip) {                                      // the norm and the factor; the Adam kernel scales as it reads
+    char* ws = (char*)tr->grad_table + trebi_grad_set_bytes(1, &tr->grad_set.total);
+    GradP p{};
+    if (int e = grad_args(tr->ctx, &tr->grad_set, tr->grad_table, 0, 1.f, ws, trebi_grad_workspace_bytes(&tr->grad_set), &p)) return e;
+    p.max_norm = max_norm;
+    p.norm_out = norm_out;
+    float* c = (float*)(ws + trebi_grad_workspace_bytes(&tr->grad_set));
+    HIPCHK(launch_grad_partials(p, st));
+    HIPCHK(launch_grad_finish(p, c, st));
+    coef = c;
+  }
   const double bc1 = 1.0 - std::pow((double)beta1, (double)adam_step);
   const double bc2 = 1.0 - std::pow((double)beta2, (double)adam_step);
   HIPCHK(launch_adam_ema(tr->params, tr->grads, tr->m, tr->v, tr->ema, tr->pi.total, beta1, beta2, (float)(lr / bc1),
-                         (float)(1.0 / std::sqrt(bc2)), eps, ema_mode, ema_decay, st));
+                         (float)(1.0 / std::sqrt(bc2)), eps, ema_mode, ema_decay, coef, st));
   return trainer_repack(tr, st);
+}
+
+extern "C" int trebi_trainer_step(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps,
+                                  int ema_mode, float ema_decay, void* stream) {
+  return trainer_step(tr, adam_step, lr, beta1, beta2, eps, ema_mode, ema_decay, false, 0.f, nullptr, (hipStream_t)stream);
+}
+
+extern "C" int trebi_trainer_step_clipped(trebi_trainer* tr, int64_t adam_step, float lr, float beta1, float beta2, float eps,
+                                          int ema_mode, float ema_decay, float max_norm, float* norm_out, void* stream) {
+  return trainer_step(tr, adam_step, lr, beta1, beta2, eps, ema_mode, ema_decay, true, max_norm, norm_out, (hipStream_t)stream);
 }

@@ -2447,14 +2447,14 @@ extern "C" double trebi_net_flops(const trebi_net* net, int backward) {
 }
 
 // ------------------------------------------------------------------------------------
+// fine-tuning operators: host side
+// ------------------------------------------------------------------------------------
+#include "finetune.inl"
+
+// ------------------------------------------------------------------------------------
 // the training step: host side
 // ------------------------------------------------------------------------------------
 #ifdef TREBI_STAMPS
 extern "C" int trebi_debug_read_wstamps(unsigned long long* out);
 #endif
 #include "trainer.inl"
-
-// ------------------------------------------------------------------------------------
-// fine-tuning operators: host side
-// ------------------------------------------------------------------------------------
-#include "finetune.inl"

@@ -143,6 +143,10 @@ SIGNATURES = {
     'trebi_trainer_accumulate': (C.c_int, [_VP, _VP, C.POINTER(_VP), _VP, _VP, C.c_int, C.c_float, _VP, _VP]),
     'trebi_trainer_step': (C.c_int, [_VP, C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int, C.c_float,
                                      _VP]),
+    'trebi_trainer_step_clipped': (C.c_int, [_VP, C.c_int64, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int, C.c_float,
+                                             C.c_float, _VP, _VP]),
+    'trebi_trainer_forward': (C.c_int, [_VP, _VP, _VP, _VP, C.c_int, _VP]),
+    'trebi_trainer_backward': (C.c_int, [_VP, _VP, _VP, _VP, C.c_int, _VP]),
     'trebi_grad_set_bytes': (C.c_size_t, [C.c_int, c_i64_p]),
     'trebi_grad_set_fill': (C.c_int, [C.c_int, C.POINTER(_VP), c_i64_p, C.POINTER(C.c_int), _VP, C.c_size_t, _VP]),
     'trebi_grad_workspace_bytes': (C.c_size_t, [_VP]),

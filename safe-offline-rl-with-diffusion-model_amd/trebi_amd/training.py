@@ -143,12 +143,128 @@ class TrainEngine:
                                                        B, float(grad_scale), _lib.ptr(out), self._stream()))
         return out
 
-    def step(self, adam_step, lr, betas=(0.9, 0.999), eps=1e-8, ema_mode=0, ema_decay=0.995):
-        _lib.check(_lib.lib().trebi_trainer_step(self.h, int(adam_step), float(lr), float(betas[0]), float(betas[1]),
-                                                 float(eps), int(ema_mode), float(ema_decay), self._stream()))
+    # ---- fine-tuning: losses over the log-probabilities of denoise transitions (trebi_amd/losses.py) ----
+    def forward(self, x, t):
+        """pred = unet(x, t) [B, H, D], with what backward() reads kept: B up to max_batch, x as the net is to see it."""
+        B = x.shape[0]
+        if x.shape != (B, self.diffusion.horizon, self.diffusion.transition_dim) or t.shape != (B,):
+            raise RuntimeError('x must be [batch, horizon, transition_dim] and t [batch]')
+        x = x.to(self.device, torch.float32).contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+        t = t.to(self.device, torch.int64).contiguous()
+        pred = torch.empty_like(x)
+        self._kept = None
+        if B:
+            _lib.check(_lib.lib().trebi_trainer_forward(self.h, _lib.ptr(x), _lib.ptr(t), _lib.ptr(pred), B, self._stream()))
+            self._kept = (x, t)                               # the backward reads them again
+        return pred
+
+    def backward(self, grad_pred):
+        """grads += (d pred / d params)^T grad_pred, for the last forward(); once per forward()."""
+        if grad_pred.shape[0] == 0:
+            return
+        if getattr(self, '_kept', None) is None:
+            raise RuntimeError('backward() follows forward(), once')
+        x, t = self._kept
+        g = grad_pred.to(self.device, torch.float32).contiguous()
+        if g.shape != x.shape:
+            raise RuntimeError(f'grad_pred has shape {tuple(g.shape)}, the forward\'s output {tuple(x.shape)}')
+        if g.data_ptr() % 16:
+            g = g.clone()
+        _lib.check(_lib.lib().trebi_trainer_backward(self.h, _lib.ptr(x), _lib.ptr(t), _lib.ptr(g), x.shape[0], self._stream()))
+        self._kept = None
+
+    def _transitions(self, x, x_prev, t):
+        """[rows, steps, H, D] (or [rows, H, D]: one step) and [rows, steps], [steps] or [rows] timesteps -> flat [B, H, D] x and
+        x_prev, [B] t, the rows' shape."""
+        x, x_prev = torch.as_tensor(x, device=self.device), torch.as_tensor(x_prev, device=self.device)
+        if x.dim() not in (3, 4) or x.shape != x_prev.shape:
+            raise RuntimeError(f'x and x_prev must be [rows, steps, horizon, transition_dim] alike, got {tuple(x.shape)} and {tuple(x_prev.shape)}')
+        lead = tuple(x.shape[:-2])
+        t = torch.as_tensor(t)
+        if not t.is_cuda and t.numel() and not (0 <= int(t.min()) and int(t.max()) < self.diffusion.n_timesteps):
+            raise RuntimeError(f'timesteps must lie in [0, {self.diffusion.n_timesteps})')
+        t = t.to(self.device, torch.int64).expand(lead).reshape(-1)
+        flat = lambda v: v.reshape(-1, *v.shape[-2:]).to(torch.float32).contiguous()
+        return flat(x), flat(x_prev), t, lead
+
+    def _parts(self, B):
+        return [(lo, min(lo + self.max_batch, B)) for lo in range(0, B, self.max_batch)]
+
+    def _fine_tune(self, x, x_prev, t, loss):
+        """Log-probabilities of all transitions (micro-batches of max_batch), `loss` on them (-> an object with .grad), and its
+        gradient back through the net.  The last micro-batch's forward serves its backward too; the others run again."""
+        from .losses import transition_log_prob, transition_log_prob_grad
+        m = self.diffusion
+        x, x_prev, t, lead = self._transitions(x, x_prev, t)
+        parts = self._parts(len(x))
+        logp, pred = [], None
+        for lo, hi in parts:
+            pred = self.forward(x[lo:hi], t[lo:hi])
+            logp.append(transition_log_prob(m, pred, x[lo:hi], x_prev[lo:hi], t[lo:hi], self.cond_keys))
+        logp = torch.cat(logp) if logp else torch.empty(0, device=self.device)
+        out = loss(logp.view(lead), (t > 0).view(lead))       # the last step (t = 0) adds no noise: nothing to learn from
+        g = out.grad.reshape(-1)
+        for k, (lo, hi) in enumerate(reversed(parts)):
+            if k:
+                pred = self.forward(x[lo:hi], t[lo:hi])
+            self.backward(transition_log_prob_grad(m, pred, x[lo:hi], x_prev[lo:hi], t[lo:hi], g[lo:hi], self.cond_keys))
+        return out, logp.view(lead)
+
+    @torch.no_grad()
+    def log_prob(self, x, x_prev, t):
+        """log p(x_prev | x) of recorded transitions under the current parameters, shaped like the rows (see _transitions): what
+        a policy step takes as logp_old / logp_ref.  chain[:, :-1], chain[:, 1:] and t = T-1 .. 0 are the transitions of a chain
+        that p_sample_loop(return_chain=True) returned with default_sample_fn (a guide moves x between the steps)."""
+        from .losses import transition_log_prob
+        x, x_prev, t, lead = self._transitions(x, x_prev, t)
+        out = [transition_log_prob(self.diffusion, self.forward(x[lo:hi], t[lo:hi]), x[lo:hi], x_prev[lo:hi], t[lo:hi], self.cond_keys)
+               for lo, hi in self._parts(len(x))]
+        self._kept = None
+        return (torch.cat(out) if out else torch.empty(0, device=self.device)).view(lead)
+
+    @torch.no_grad()
+    def accumulate_policy(self, x, x_prev, t, advantages, logp_old=None, logp_ref=None, *, mask=None, grad_scale=1.0, **loss):
+        """grads += grad_scale * d policy_loss / d params over recorded transitions (losses.policy_loss's keywords: clip,
+        clip_high, dual_clip, kl_coef, kl, reduction, denominator, per_token).  x, x_prev: [rows, steps, H, D]; t: [rows, steps]
+        or [steps]; advantages: one a row or one a step; logp_old / logp_ref / mask: [rows, steps].  Steps at t = 0 do not
+        count.  Returns (PolicyLoss, logp [rows, steps])."""
+        from .losses import policy_loss
+        like = lambda v: None if v is None else torch.as_tensor(v, device=self.device, dtype=torch.float32)
+
+        def one(logp, noisy):
+            keep = noisy if mask is None else noisy & (torch.as_tensor(mask, device=self.device) != 0)
+            return policy_loss(logp, like(advantages), like(logp_old), like(logp_ref), mask=keep, grad_scale=grad_scale, **loss)
+        return self._fine_tune(x, x_prev, t, one)
+
+    @torch.no_grad()
+    def accumulate_preference(self, x, x_prev, t, logp_ref=None, *, mask=None, grad_scale=1.0, **loss):
+        """grads += grad_scale * d preference_loss / d params (losses.preference_loss's keywords).  Rows k < rows / 2 of x, x_prev
+        [rows, steps, H, D] are preferred to rows k + rows / 2; logp_ref [rows, steps]: log_prob() under the reference
+        parameters.  Steps at t = 0 do not count.  Returns (PreferenceLoss, logp [rows, steps])."""
+        from .losses import preference_loss
+        ref = None if logp_ref is None else torch.as_tensor(logp_ref, device=self.device, dtype=torch.float32)
+
+        def one(logp, noisy):
+            keep = noisy if mask is None else noisy & (torch.as_tensor(mask, device=self.device) != 0)
+            return preference_loss(logp, ref, mask=keep, grad_scale=grad_scale, **loss)
+        return self._fine_tune(x, x_prev, t, one)
+
+    def step(self, adam_step, lr, betas=(0.9, 0.999), eps=1e-8, ema_mode=0, ema_decay=0.995, max_grad_norm=None):
+        """optimizer.step() and the EMA copy; with max_grad_norm the gradient is clipped to that global norm first, inside the
+        same pass, and its norm before clipping returned (a device scalar)."""
+        args = (self.h, int(adam_step), float(lr), float(betas[0]), float(betas[1]), float(eps), int(ema_mode), float(ema_decay))
+        norm = None
+        if max_grad_norm is None:
+            _lib.check(_lib.lib().trebi_trainer_step(*args, self._stream()))
+        else:
+            norm = torch.empty((), device=self.device)
+            _lib.check(_lib.lib().trebi_trainer_step_clipped(*args, float(max_grad_norm), _lib.ptr(norm), self._stream()))
         for net in (self.unet, getattr(self, 'ema_unet', None)):      # planning with these modules must re-pack
             if net is not None:
                 net._packed_key = None
+        return norm
 
     def __del__(self):
         try:
@@ -185,12 +301,15 @@ class Trainer:
     bucket (up path, mid blocks, final conv: the first gradients the backward finishes) goes out on a side stream
     while the last micro-batch's down-path backward still runs, the head bucket after it.  Each micro-batch is
     scaled by B_local / B_global so that the sum equals the gradient of the mean loss over the global batch.
+    max_grad_norm: clip the (reduced) gradient to that global norm in every step; `grad_norm` then holds the last one.
+    policy_step / preference_step fine-tune on recorded transitions instead (no counterpart in the reference).
     `engine_factory` exists so that the distributed logic can be exercised on CPU ranks (gloo) without a GPU."""
 
     def __init__(self, diffusion_model, dataset=None, renderer=None, ema_decay=0.995, train_batch_size=32, train_lr=2e-5,
                  gradient_accumulate_every=2, step_start_ema=2000, update_ema_every=10, log_freq=100, sample_freq=1000,
                  save_freq=1000, label_freq=100000, save_parallel=False, results_folder='./results', n_reference=8,
-                 bucket=None, group=None, distributed=None, engine_factory=None, adam_betas=(0.9, 0.999), adam_eps=1e-8):
+                 bucket=None, group=None, distributed=None, engine_factory=None, adam_betas=(0.9, 0.999), adam_eps=1e-8,
+                 max_grad_norm=None):
         self.model = diffusion_model
         self.ema_decay = ema_decay
         self.update_ema_every = update_ema_every
@@ -199,6 +318,7 @@ class Trainer:
         self.batch_size = train_batch_size
         self.gradient_accumulate_every = gradient_accumulate_every
         self.lr, self.betas, self.eps = train_lr, adam_betas, adam_eps
+        self.max_grad_norm, self.grad_norm = max_grad_norm, None
         self.dataset = dataset
         self.logdir = results_folder
         self.group = group
@@ -261,29 +381,63 @@ class Trainer:
                 self._side.wait_event(self._bucket_event)
                 with torch.cuda.stream(self._side):        # the tail bucket leaves while the down path's backward runs
                     tail_work = dist.all_reduce(g[split:], op=dist.ReduceOp.SUM, group=self.group, async_op=True)
-        if world > 1:
-            def reduce(v):
-                if through_host:                           # gloo (CPU rehearsals): through the host
-                    vh = v.cpu()
-                    dist.all_reduce(vh, op=dist.ReduceOp.SUM, group=self.group)
-                    v.copy_(vh)
-                else:
-                    dist.all_reduce(v, op=dist.ReduceOp.SUM, group=self.group)
-            if tail_work is not None:
-                reduce(g[:split])
-                tail_work.wait()                           # the current stream waits for the side stream's collective
-            elif split:
-                reduce(g[split:])
-                reduce(g[:split])
+        if tail_work is not None:
+            self._reduce(g[:split])
+            tail_work.wait()                               # the current stream waits for the side stream's collective
+        else:
+            self._reduce_all()
+        self._optimiser_step()
+        return losses
+
+    def _reduce(self, v):
+        if v.is_cuda and dist.get_backend(self.group) == 'gloo':                        # CPU rehearsals: through the host
+            vh = v.cpu()
+            dist.all_reduce(vh, op=dist.ReduceOp.SUM, group=self.group)
+            v.copy_(vh)
+        else:
+            dist.all_reduce(v, op=dist.ReduceOp.SUM, group=self.group)
+
+    def _reduce_all(self):
+        if self._world() > 1:
+            g = self.engine.grads
+            split = int(getattr(self.engine, 'bucket_split', 0))
+            if 0 < split < g.numel():
+                self._reduce(g[split:])
+                self._reduce(g[:split])
             else:
-                reduce(g)
+                self._reduce(g)
+
+    def _optimiser_step(self):
         self.adam_steps += 1
         ema_mode = 0
         if self.step % self.update_ema_every == 0:                                      # training.py:121-122, 94-98
             ema_mode = 1 if self.step < self.step_start_ema else 2
-        self.engine.step(self.adam_steps, self.lr, self.betas, self.eps, ema_mode, self.ema_decay)
+        clip = {} if self.max_grad_norm is None else dict(max_grad_norm=self.max_grad_norm)
+        self.grad_norm = self.engine.step(self.adam_steps, self.lr, self.betas, self.eps, ema_mode, self.ema_decay, **clip)
         self.step += 1
-        return losses
+
+    def _fine_tune_step(self, accumulate, batches, global_rows):
+        """One optimiser step over `batches` of accumulate_policy's / accumulate_preference's arguments.  Data-parallel: every rank
+        brings its own rows; each micro-batch counts rows_local / rows_global (give `denominator` for another weighting)."""
+        world, out = self._world(), []
+        for i, batch in enumerate(batches):
+            batch = dict(batch)
+            rows = len(batch['x'])
+            total = global_rows[i] if global_rows is not None else rows * world
+            share = 1.0 if batch.get('denominator') is not None else (rows / total if total else 0.0)
+            out.append(accumulate(**batch, grad_scale=share / len(batches))[0])
+        self._reduce_all()
+        self._optimiser_step()
+        return out
+
+    def policy_step(self, batches, global_rows=None):
+        """One clipped-policy-gradient step: `batches` are dicts of TrainEngine.accumulate_policy's arguments (x, x_prev, t,
+        advantages, logp_old, ...).  Returns the per-micro-batch PolicyLoss (device, no host sync)."""
+        return self._fine_tune_step(self.engine.accumulate_policy, batches, global_rows)
+
+    def preference_step(self, batches, global_rows=None):
+        """One preference step: dicts of TrainEngine.accumulate_preference's arguments (x, x_prev, t, logp_ref, ...)."""
+        return self._fine_tune_step(self.engine.accumulate_preference, batches, global_rows)
 
     def train(self, n_train_steps):                                                     # training.py:104-139
         if self.dataloader is None:
