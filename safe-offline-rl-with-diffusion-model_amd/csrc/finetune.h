@@ -1,4 +1,4 @@
-// Kernel arguments and launchers of the fine-tuning operators (gradnorm.hip, policy.hip, pairs.hip, transition.hip), shared with the host side
+// Kernel arguments and launchers of the fine-tuning operators (gradnorm.hip, policy.inl, policy.hip, pairs.hip, transition.hip), shared with the host side
 // (finetune.inl).
 #pragma once
 #include <hip/hip_runtime.h>
@@ -36,7 +36,7 @@ struct TokenP {
 };
 struct NormPart { long long tokens, rows; };
 constexpr int COUNT_BLOCKS = 256;          // partial counts
-constexpr int LOSS_PARTS = 1280;          // workgroups of the policy loss at most: the 5 that fit on each CU at once
+constexpr int LOSS_PARTS = 1280;          // partial sums the policy loss may leave
 constexpr int LOSS_VALS = 5;
 
 struct PolicyP {
@@ -60,6 +60,7 @@ struct PolicyP {
   double* weight;                          // the weight, from the loss kernel to the one that finishes
   float* stats;                            // [5]
   long long per;                           // tokens of a workgroup
+  int early;                               // load tokens before it is known which of them count
   int flat;                                // every view is contiguous and rows are not tiny: vector loads across rows
 };
 hipError_t launch_token_counts(const PolicyP& p, hipStream_t st);

@@ -92,8 +92,10 @@ int token_args(const trebi_token_desc& d, TokenP* t) {
   return 0;
 }
 
-// policy workspace: partial counts, partial sums, a count for each row
+// policy workspace: partial counts, partial sums, a count for each row; a call of one workgroup without a mask needs none
+constexpr long long SINGLE = 4096;
 size_t policy_bytes(const trebi_token_desc& d) {
+  if (!d.mask && d.rows >= 0 && d.rows <= SINGLE && d.len >= 0 && (d.packed || d.len <= SINGLE) && (d.packed ? d.len : d.rows * d.len) <= SINGLE) return 0;
   return al256(COUNT_BLOCKS * sizeof(NormPart)) + al256((LOSS_PARTS * LOSS_VALS + 1) * sizeof(double)) +
          (d.mask ? al256((size_t)d.rows * sizeof(int)) : 0);
 }
@@ -106,8 +108,20 @@ int pair_splits(const trebi_token_desc& d) {
   if (d.rows / 2 >= 512 || len <= 4096) return 0;
   return (int)std::max<long long>(1, std::min<long long>(PAIR_BLOCKS / d.rows, (len + 4095) / 4096));
 }
+// Threads of a pair: at most two turns of 16 tokens each, on average
+int pair_group(const trebi_token_desc& d) {
+  const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len;
+  return len <= 128 ? 16 : len <= 512 ? 64 : 256;
+}
+int pair_blocks(const trebi_token_desc& d) {
+  const int g = pair_group(d), per = 256 / g;
+  return (int)std::min<long long>(PAIR_BLOCKS, (d.rows / 2 + per - 1) / per);
+}
+// preference workspace: partial sums, the rows' parts; a call of one workgroup needs none
 size_t pair_bytes(const trebi_token_desc& d) {
+  if (d.rows < 2) return 0;
   const int s = pair_splits(d);
+  if (!s && pair_blocks(d) == 1) return 0;
   return al256(PAIR_BLOCKS * 4 * sizeof(double)) + (s ? al256((size_t)d.rows * s * 2 * sizeof(double)) : 0);
 }
 
@@ -200,7 +214,7 @@ extern "C" size_t trebi_policy_loss_workspace_bytes(const trebi_token_desc* d) {
 
 extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const trebi_policy_loss_desc* d, void* workspace,
                                  size_t workspace_bytes, void* stream) {
-  if (!ctx || !tokens || !d || !workspace) return fail(TREBI_BAD_ARG, "null argument");
+  if (!ctx || !tokens || !d || (!workspace && policy_bytes(*tokens))) return fail(TREBI_BAD_ARG, "null argument");
   PolicyP p{};
   if (int e = token_args(*tokens, &p.tk)) return e;
   const bool empty = p.tk.n == 0;
@@ -260,11 +274,15 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
   ON_DEVICE(ctx);
   // One workgroup does it all up to 4096 tokens (at most 4 turns): a call of this size is bound by its launches.
   const long long turn = 256 * pack, turns = (t.n + turn - 1) / turn;
-  const long long per = t.n <= 4096 ? std::max<long long>(turns, 1) : (turns + LOSS_PARTS - 1) / LOSS_PARTS;
+  // ... else as many workgroups as fit on the 256 CUs at once, so that none is left for a second round: 5 or (see the kernel) 4
+  const long long most = t.packed || p.acs || (p.ref && p.kl == 3) ? 1024 : LOSS_PARTS;
+  const long long per = t.n <= SINGLE ? std::max<long long>(turns, 1) : (turns + most - 1) / most;
   const int blocks = (int)((turns + per - 1) / per);
   p.per = per * turn;
-  if (!empty && (p.counts || (p.fixed == 0.0 && (blocks > 1 || t.mask || t.rows > 4096)))) {
-    p.nnp = (int)(t.mask ? std::min<long long>(COUNT_BLOCKS, t.rows) : std::min<long long>(16, (t.rows + 255) / 256));
+  p.early = all || (t.packed && !t.mask) || per == 1;
+  const bool told = t.packed && p.mode == 0 && !t.mask;               // the offsets say how many tokens there are
+  if (!empty && !told && (p.counts || (p.fixed == 0.0 && (blocks > 1 || t.mask || t.rows > SINGLE)))) {
+    p.nnp = (int)(t.mask ? std::min<long long>(COUNT_BLOCKS, t.rows) : std::min<long long>(COUNT_BLOCKS, (t.rows + 255) / 256));
     HIPCHK(launch_token_counts(p, st));
   }
   if (!empty) HIPCHK(launch_policy(p, d->dtype, blocks, st));
@@ -276,11 +294,11 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
 // ---------------------------------------------------------------------------------------------------------------
 // preference loss
 // ---------------------------------------------------------------------------------------------------------------
-extern "C" size_t trebi_preference_loss_workspace_bytes(const trebi_token_desc* d) { return d && d->rows > 0 ? pair_bytes(*d) : 256; }
+extern "C" size_t trebi_preference_loss_workspace_bytes(const trebi_token_desc* d) { return d ? pair_bytes(*d) : 0; }
 
 extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const trebi_preference_loss_desc* d,
                                      void* workspace, size_t workspace_bytes, void* stream) {
-  if (!ctx || !tokens || !d || !workspace) return fail(TREBI_BAD_ARG, "null argument");
+  if (!ctx || !tokens || !d) return fail(TREBI_BAD_ARG, "null argument");
   PairP p{};
   if (int e = token_args(*tokens, &p.tk)) return e;
   if (p.tk.rows < 2 || p.tk.rows % 2) return fail(TREBI_BAD_SHAPE, "%lld rows: chosen and rejected rows come in pairs", (long long)p.tk.rows);
@@ -290,6 +308,7 @@ extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tok
   if (!(d->beta > 0.f)) return fail(TREBI_BAD_ARG, "beta must be positive");
   if (!(d->label_smoothing >= 0.f) || !(d->label_smoothing < 0.5f)) return fail(TREBI_BAD_ARG, "label_smoothing must lie in [0, 0.5)");
   if (d->denominator < 0.0 || d->denominator != d->denominator) return fail(TREBI_BAD_ARG, "denominator must be positive (0: the number of pairs)");
+  if (!workspace && pair_bytes(*tokens)) return fail(TREBI_BAD_ARG, "workspace is null");
   if (workspace_bytes < pair_bytes(*tokens)) return fail(TREBI_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, pair_bytes(*tokens));
   p.pairs = p.tk.rows / 2;
   p.lp = d->logp; p.ref = d->logp_ref;
@@ -312,10 +331,8 @@ extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tok
     p.nparts = (int)p.pairs;
     HIPCHK(launch_pairs_split(p, d->dtype, st));
   } else {
-    const long long len = p.tk.packed ? (p.tk.n + p.tk.rows - 1) / p.tk.rows : p.tk.len;
-    p.group = len <= 128 ? 16 : len <= 512 ? 64 : 256;            // at most two turns of 16 tokens a thread, on average
-    const long long per = 256 / p.group;
-    const int blocks = (int)std::min<long long>(PAIR_BLOCKS, (p.pairs + per - 1) / per);
+    p.group = pair_group(*tokens);
+    const int blocks = pair_blocks(*tokens);
     p.nparts = blocks;
     HIPCHK(launch_pairs_whole(p, d->dtype, blocks, st));
   }

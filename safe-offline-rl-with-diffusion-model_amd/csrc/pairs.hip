@@ -187,7 +187,8 @@ __global__ __launch_bounds__(256) void pairs_whole_kernel(PairP p) {
       }
       o[0] = __shfl_xor(v[0], half, 64);
       o[1] = __shfl_xor(v[1], half, 64);
-    } else {                                          // two waves a row
+    } else {                                          // the workgroup takes one pair, half of its waves a row
+      constexpr int HW = 2;
       __syncthreads();
       v[0] = wave_sum64(v[0]);
       v[1] = wave_sum64(v[1]);
@@ -196,15 +197,19 @@ __global__ __launch_bounds__(256) void pairs_whole_kernel(PairP p) {
         lds[(threadIdx.x >> 6) * 2 + 1] = v[1];
       }
       __syncthreads();
-      const int w = second ? 4 : 0;
-      v[0] = lds[w] + lds[w + 2];
-      v[1] = lds[w + 1] + lds[w + 3];
-      o[0] = lds[4 - w] + lds[6 - w];
-      o[1] = lds[5 - w] + lds[7 - w];
+      const int mine = second ? 2 * HW : 0, other = 2 * HW - mine;
+      v[0] = v[1] = o[0] = o[1] = 0.0;
+#pragma unroll
+      for (int w = 0; w < HW; ++w) {
+        v[0] += lds[mine + 2 * w];
+        v[1] += lds[mine + 2 * w + 1];
+        o[0] += lds[other + 2 * w];
+        o[1] += lds[other + 2 * w + 1];
+      }
     }
     if (on) {
       float rc, rr;
-      const PairOut q = second ? pair_math(p, k, o[0], o[1], v[0], v[1], &rc, &rr) : pair_math(p, k, v[0], v[1], o[0], o[1], &rc, &rr);
+      const PairOut q = pair_math(p, k, second ? o[0] : v[0], second ? o[1] : v[1], second ? v[0] : o[0], second ? v[1] : o[1], &rc, &rr);
       if (lane == 0 && !second) {
         p.rew_c[k] = rc;
         p.rew_r[k] = rr;
@@ -247,16 +252,16 @@ __global__ __launch_bounds__(256) void pairs_sum_kernel(PairP p) {
 }
 template <typename T>
 __global__ __launch_bounds__(256) void pairs_grad_kernel(PairP p) {
-  __shared__ double lds[20];
   const long long r = blockIdx.x / p.splits;
   const int j = blockIdx.x - (int)r * p.splits;
   const long long k = r < p.pairs ? r : r - p.pairs;
-  double v[4] = {0, 0, 0, 0};
-  for (int i = threadIdx.x; i < p.splits; i += 256) {
+  double v[4] = {0, 0, 0, 0};                          // every wave adds the splits' sums up for itself: no barrier
+  for (int i = threadIdx.x & 63; i < p.splits; i += 64) {
     const double *c = p.rowpart + (k * p.splits + i) * 2, *q = p.rowpart + ((k + p.pairs) * p.splits + i) * 2;
     v[0] += c[0]; v[1] += c[1]; v[2] += q[0]; v[3] += q[1];
   }
-  block_sum<4, 256>(v, lds);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = wave_sum64(v[q]);
   float rc, rr;
   const PairOut o = pair_math(p, k, v[0], v[1], v[2], v[3], &rc, &rr);
   if (r < p.pairs && j == 0 && threadIdx.x == 0) {

@@ -1,8 +1,5 @@
-// Clipped policy loss with a KL term, and its gradient.
-//
-// Bound by memory: a token costs 2..4 loads, one store and some tens of instructions.  Inputs are read once and the
-// gradient leaves in the same pass; scalars are summed in float64 per workgroup, in a fixed order, and a one-workgroup
-// kernel adds the workgroups' partial sums (no atomics: results do not change from run to run).
+// Clipped policy loss with a KL term: token counts, the sum of the workgroups' parts, and which kernel a call takes (the kernels
+// themselves: policy.inl).
 #include "finetune.h"
 #include "tokens.h"
 
@@ -60,470 +57,6 @@ __global__ __launch_bounds__(256) void token_count_kernel(TokenP t, int G, NormP
   if (threadIdx.x == 0) np[blockIdx.x] = {(long long)v[0], (long long)v[1]};
 }
 
-// ---------------------------------------------------------------------------------------------------------------
-// Clipped policy loss with a KL term
-//   d = logp - old, rho = e^d;  beyond a border in the direction that the advantage A pushes, the ratio is held there
-//   and the token gives no gradient:   A > 0: d > log(1 + eps_high);  A < 0: d < log(1 - eps_low), or d > log(dual)
-//   pg = -A rho;  delta = ref - logp;  kl = -delta | delta^2 / 2 | e^delta - delta - 1
-//   loss = sum_i w_i (pg_i + beta kl_i)
-// A thread takes N = 16 bytes of consecutive tokens (4 or 8).  N tokens of rows of at least N lie in at most two rows, so
-// what belongs to a row (advantage, borders, weight) is looked up twice, not N times, and a wave whose tokens all count and
-// lie in one row runs without any selection: with 8 bytes a token (bfloat16) it is the instructions that would bound this
-// kernel.  Which row that is goes through the scalar cache, beside the loads of the tokens themselves; for packed sequences
-// the wave looks for it 64 offsets at a time (two loads for 4096 sequences, where halving takes twelve).
-// A token's side of a border must not hang on a rounding.  d is rounded to float32, which cannot carry it past the
-// border's own float32 value but can make the two equal; only then the comparison is made again in float64, where the
-// difference is exact for every input type.
-// ---------------------------------------------------------------------------------------------------------------
-struct PolicyAcc { float pg, kl, rho; unsigned cut; };
-
-// e^x by the exponential unit: within (|x| + 2) 2^-24 of e^x, which the rounding of the difference x (|x| 2^-24) allows for
-__device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
-
-// e^x - 1 and e^x - x - 1 without cancellation: the series below |x| = 1 (its 12th term is under 2^-24 of the sum)
-__device__ __forceinline__ void exp_parts(float x, float* em1, float* rest) {
-  float q = 1.f / 479001600.f;
-  q = fmaf(q, x, 1.f / 39916800.f);
-  q = fmaf(q, x, 1.f / 3628800.f);
-  q = fmaf(q, x, 1.f / 362880.f);
-  q = fmaf(q, x, 1.f / 40320.f);
-  q = fmaf(q, x, 1.f / 5040.f);
-  q = fmaf(q, x, 1.f / 720.f);
-  q = fmaf(q, x, 1.f / 120.f);
-  q = fmaf(q, x, 1.f / 24.f);
-  q = fmaf(q, x, 1.f / 6.f);
-  q = fmaf(q, x, 0.5f);
-  float r = x * x * q, m = r + x;
-  if (!(fabsf(x) < 1.f)) {
-    const float e = exp_near(x);
-    m = e - 1.f;
-    r = m - x;
-  }
-  *em1 = m;
-  *rest = r;
-}
-
-// The KL term of x = ref - logp and its derivative by logp; KL 0: none, 1..3: the kinds
-template <int KL>
-__device__ __forceinline__ void kl_term(float x, float* kl, float* dk) {
-  *kl = *dk = 0.f;
-  if (KL == 1) { *kl = -x; *dk = 1.f; }
-  if (KL == 2) { *kl = 0.5f * x * x; *dk = -x; }
-  if (KL == 3) { float m; exp_parts(x, &m, kl); *dk = -m; }
-}
-
-// Is the token beyond a border (from the difference in float64), and the ratio that is held there
-__device__ __forceinline__ bool beyond(const PolicyP& p, float lp, float old, float A, float* held) {
-  const double x = (double)lp - (double)old;
-  const float vhi = p.vhi, vlo = p.vlo, vdual = p.vdual;
-  const bool over = A > 0.f && x > p.hi, far = A < 0.f && x > p.dual, under = A < 0.f && x < p.lo;
-  *held = over ? vhi : (under ? vlo : vdual);
-  return over || far || under;
-}
-
-// One token.  Returns the gradient before its weight; bit `e` of a.cut says whether it is beyond a border.
-template <int KL>
-__device__ __forceinline__ float policy_token(const PolicyP& p, float lp, float old, float ref, float A, float u, int e, PolicyAcc& a) {
-  // (by value: a selection between fields of the kernel's arguments would be one of addresses, and put them into scratch)
-  const float fhi = p.fhi, flo = p.flo, fdual = p.fdual, vhi = p.vhi, vlo = p.vlo, vdual = p.vdual;
-  const float d = lp - old;
-  float held = A > 0.f ? vhi : (d > 0.f ? vdual : vlo);
-  bool cut = A > 0.f ? d > fhi : (A < 0.f && (d < flo || d > fdual));
-  if (d == fhi || d == flo || d == fdual) cut = beyond(p, lp, old, A, &held);
-  const float rho = exp_near(d);
-  const float pg = -A * (cut ? held : rho);
-  float g = cut ? 0.f : pg;
-  if (KL) {
-    float kl, dk;
-    kl_term<KL>(ref - lp, &kl, &dk);
-    g = fmaf(p.kl_coef, dk, g);
-    a.kl = fmaf(u, kl, a.kl);
-  }
-  a.pg = fmaf(u, pg, a.pg);
-  a.rho += rho;
-  a.cut |= cut ? 1u << e : 0u;
-  return g;
-}
-
-// What multiplies a token besides 1 / (its row's length): 1 / tokens, 1 / sequences or 1 / denominator.
-__device__ __forceinline__ double policy_weight(const PolicyP& p, double tokens, double rows) {
-  if (p.fixed > 0.0) return p.fixed;
-  const double n = p.mode == 0 ? tokens : rows;
-  return n > 0.0 ? 1.0 / n : 0.0;
-}
-// ... from the partial counts, or (one workgroup, no mask) from the rows themselves
-template <int NT>
-__device__ __forceinline__ double policy_weight_parts(const PolicyP& p, double* lds) {
-  if (p.fixed > 0.0) return p.fixed;
-  double v[2] = {0, 0};
-  if (p.nnp > 0 && p.nnp <= 16) {
-    for (int i = 0; i < p.nnp; ++i) {
-      const NormPart q = uniform_load(p.np + i);
-      v[0] += (double)q.tokens;
-      v[1] += (double)q.rows;
-    }
-    return policy_weight(p, v[0], v[1]);
-  }
-  if (p.nnp == 0) {
-    for (long long r = threadIdx.x; r < p.tk.rows; r += NT) {
-      long long s, e;
-      row_bounds(p.tk, r, &s, &e);
-      v[0] += (double)(e - s);
-      v[1] += e > s ? 1.0 : 0.0;
-    }
-  } else {
-    for (int i = threadIdx.x; i < p.nnp; i += NT) {
-      v[0] += (double)p.np[i].tokens;
-      v[1] += (double)p.np[i].rows;
-    }
-  }
-  block_sum<2, NT>(v, lds);
-  return policy_weight(p, v[0], v[1]);
-}
-
-// The last sequence that begins at or before token i (its first one is 0), searched in [lo, hi].
-__device__ __forceinline__ int find_row(const int* cu, int lo, int hi, long long i) {
-  while (lo < hi) {
-    const int m = lo + ((hi - lo + 1) >> 1);
-    if ((long long)cu[m] <= i) lo = m;
-    else hi = m - 1;
-  }
-  return lo;
-}
-// The same for a token that is the same in the whole wave, by its 64 lanes (all of them active)
-__device__ __forceinline__ int find_row_wave(const int* cu, int rows, long long i) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = rows;
-  while (n > 1) {
-    const int step = (n + 63) >> 6;
-    const int at = lane * step;
-    const bool le = at < n && (long long)cu[lo + (at < n ? at : 0)] <= i;
-    const int c = __popcll(__ballot(le));
-    if (c == 0) return lo;
-    lo += (c - 1) * step;
-    n = min(step, n - (c - 1) * step);
-  }
-  return lo;
-}
-
-// What a row's tokens share
-struct RowInfo { float A, u; };
-__device__ __forceinline__ RowInfo row_info(const PolicyP& p, long long r, long long tokens) {
-  RowInfo ri{p.acs ? 0.f : p.adv[r * p.ars], 1.f};
-  if (p.mode == 1) {
-    const long long c = p.counts ? (long long)p.counts[r] : tokens;
-    ri.u = c > 0 ? 1.f / (float)c : 0.f;
-  }
-  return ri;
-}
-
-struct PolicySum { double pg, kl, rho; long long cut, cnt; };
-
-__device__ __forceinline__ long long row_of(const TokenP& t, long long i) {
-  return t.n <= 0xffffffffll ? (long long)((unsigned)i / (unsigned)t.len) : i / t.len;
-}
-
-// Token i, whatever the views' strides and the rows' lengths
-template <typename T>
-__device__ __forceinline__ void policy_one(const PolicyP& p, long long i, float W, PolicySum& sum) {
-  long long r, c, s, e;
-  if (p.tk.packed) {
-    r = find_row(p.tk.cu, 0, (int)p.tk.rows - 1, i);
-    c = i;
-  } else {
-    r = row_of(p.tk, i);
-    c = i - r * p.tk.len;
-  }
-  row_bounds(p.tk, r, &s, &e);
-  bool valid = c >= s && c < e;
-  if (valid && p.tk.mask) valid = p.tk.mask[(p.tk.packed ? 0 : r * p.tk.mrs) + c * p.tk.mcs] != 0;
-  float g = 0.f;
-  if (valid) {
-    const RowInfo ri = row_info(p, r, e - s);
-    const long long k = p.tk.packed ? 0 : r;
-    const float lp = load_one((const T*)p.lp + k * p.lrs + c * p.lcs);
-    const float old = p.old ? load_one((const T*)p.old + k * p.ors + c * p.ocs) : lp;
-    const float ref = p.ref ? load_one((const T*)p.ref + k * p.rrs + c * p.rcs) : 0.f;
-    const float A = p.acs ? p.adv[k * p.ars + c * p.acs] : ri.A;
-    PolicyAcc a{0, 0, 0, 0};
-    g = !p.ref ? policy_token<0>(p, lp, old, ref, A, ri.u, 0, a) : p.kl == 1 ? policy_token<1>(p, lp, old, ref, A, ri.u, 0, a)
-      : p.kl == 2 ? policy_token<2>(p, lp, old, ref, A, ri.u, 0, a) : policy_token<3>(p, lp, old, ref, A, ri.u, 0, a);
-    g *= W * ri.u;
-    sum.pg += (double)a.pg;
-    sum.kl += (double)a.kl;
-    sum.rho += (double)a.rho;
-    sum.cut += a.cut;
-    sum.cnt += 1;
-  }
-  if (p.grad) store_one((T*)p.grad + i, g);
-}
-
-template <typename T, int KL, bool TA, int N>
-struct PolicyLoad {
-  Pack<T, N> l, o, f;
-  Pack<float, N> a;
-  __device__ __forceinline__ void load(const PolicyP& p, long long i) {
-    l.load((const T*)p.lp + i);
-    if (p.old) o.load((const T*)p.old + i);
-    if (KL) f.load((const T*)p.ref + i);
-    if (TA) a.load(p.adv + i);
-  }
-};
-
-// The rows of a thread's tokens i .. i + N - 1: the first k1 are of row a, the others of row b; bit e of valid: token i + e
-// counts; single: more than two rows, one by one; one_row: the whole wave lies in row a.
-struct RowsOfPack { RowInfo a, b; int k1; unsigned valid; bool single, one_row; };
-__device__ __forceinline__ unsigned low_bits(int n) { return (1u << n) - 1u; }
-
-// The begins of 64 sequences from `r` on, one a lane, kept from turn to turn: the tokens of a workgroup are consecutive, so
-// most turns find their sequences without a load.
-struct Window { int r, at; };
-
-// All lanes active; iw .. lw: the wave's tokens
-template <int N>
-__device__ __forceinline__ RowsOfPack rows_packed(const PolicyP& p, Window& w, long long i, long long iw, long long lw) {
-  const TokenP& t = p.tk;
-  const int rows = (int)t.rows, lane = threadIdx.x & 63;
-  RowsOfPack q;
-  q.single = false;
-  int k = 0;                                                           // the wave's first sequence is w.r + k
-  if (w.r >= 0) k = max(0, __popcll(__ballot((long long)w.at <= iw)) - 1);
-  if (w.r < 0 || k == 63 || (w.r + 61 < rows && (long long)__builtin_amdgcn_readlane(w.at, 61) <= lw)) {
-    w.r = uniform(w.r < 0 || k == 63 ? find_row_wave(t.cu, rows, iw) : w.r + k);
-    w.at = t.cu[min(w.r + lane, rows)];                                // (behind the last one: its end)
-    k = 0;
-  }
-  k = uniform(k);
-  const int o0 = __builtin_amdgcn_readlane(w.at, k), o1 = __builtin_amdgcn_readlane(w.at, k + 1), r = w.r + k;
-  q.one_row = r < rows && o0 <= iw && lw < o1 && o1 <= t.n;
-  if (q.one_row) {
-    const long long c = p.counts && p.mode == 1 ? (long long)uniform_load(p.counts + r) : (long long)o1 - (o0 < 0 ? 0 : o0);
-    q.a = q.b = RowInfo{p.acs ? 0.f : uniform_load(p.adv + r * p.ars), p.mode != 1 ? 1.f : c > 0 ? 1.f / (float)c : 0.f};
-    q.k1 = N;
-    q.valid = low_bits(N);
-    return q;
-  }
-  if (i >= t.n) i = t.n - 1;                                           // (a lane behind the end: its answer is not used)
-  int row;
-  long long s, e, e2;
-  if (w.r + 61 < rows && (long long)__builtin_amdgcn_readlane(w.at, 61) <= lw) {       // more sequences than lanes
-    row = find_row(t.cu, w.r, rows - 1, i);
-    row_bounds(t, row, &s, &e);
-    e2 = e;
-    if (row + 1 < rows) {
-      long long s2;
-      row_bounds(t, row + 1, &s2, &e2);
-    }
-  } else {
-    int pos = 0;
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1)
-      if ((long long)__shfl(w.at, pos + step, 64) <= i) pos += step;
-    pos = min(pos, min(rows - 1 - w.r, 61));
-    row = w.r + pos;
-    s = __shfl(w.at, pos, 64);
-    e = __shfl(w.at, pos + 1, 64);
-    e2 = __shfl(w.at, pos + 2, 64);
-    s = s < 0 ? 0 : (s > t.n ? t.n : s);
-    e = e < s ? s : (e > t.n ? t.n : e);
-    e2 = e2 < e ? e : (e2 > t.n ? t.n : e2);
-  }
-  const bool two = e < i + N && row + 1 < rows;
-  q.single = i < s || (two && e2 < i + N && row + 2 < rows);
-  q.k1 = e <= i ? 0 : e - i < N ? (int)(e - i) : N;
-  q.a = q.b = row_info(p, row, e - s);
-  int nb = 0;
-  if (two) {
-    nb = e2 >= i + N ? N - q.k1 : e2 <= i + q.k1 ? 0 : (int)(e2 - i) - q.k1;
-    q.b = row_info(p, row + 1, e2 - e);
-  }
-  q.valid = low_bits(q.k1 + nb);
-  return q;
-}
-
-template <int N>
-__device__ __forceinline__ RowsOfPack rows_padded(const PolicyP& p, long long i, long long iw, long long lw) {
-  const TokenP& t = p.tk;
-  const long long L = t.len, r0 = uniform(row_of(t, iw));
-  RowsOfPack q;
-  q.single = false;
-  q.one_row = lw < (r0 + 1) * L;
-  long long s, e;
-  if (q.one_row) {
-    e = t.lengths ? (long long)uniform_load(t.lengths + r0) : L;
-    e = e < 0 ? 0 : (e > L ? L : e);
-    const long long c = i - r0 * L, m = p.mode != 1 ? 0 : p.counts ? (long long)uniform_load(p.counts + r0) : e;
-    q.a = q.b = RowInfo{p.acs ? 0.f : uniform_load(p.adv + r0 * p.ars), p.mode != 1 ? 1.f : m > 0 ? 1.f / (float)m : 0.f};
-    q.k1 = N;
-    q.valid = low_bits(e <= c ? 0 : e - c < N ? (int)(e - c) : N);
-    return q;
-  }
-  if (i >= t.n) i = t.n - 1;
-  const long long r = row_of(t, i), c = i - r * L;
-  row_bounds(t, r, &s, &e);
-  q.k1 = L - c < N ? (int)(L - c) : N;
-  q.valid = low_bits(e <= c ? 0 : e - c < q.k1 ? (int)(e - c) : q.k1);
-  q.a = q.b = row_info(p, r, e);
-  if (q.k1 < N && r + 1 < t.rows) {
-    row_bounds(t, r + 1, &s, &e);
-    q.valid |= low_bits(e < N - q.k1 ? (int)e : N - q.k1) << q.k1;
-    q.b = row_info(p, r + 1, e);
-  }
-  return q;
-}
-
-// N tokens of one row that all count, in every lane.  With s the advantage's sign a token is beyond the border where s d
-// exceeds one number (and with a dual border where -s d, s < 0, exceeds another), and what the row shares is taken out of
-// the sums.  False: some lane's rounded difference equals a border, nothing was done.
-template <typename T, int KL, bool TA, int N, bool DUAL>
-__device__ __forceinline__ bool policy_row(const PolicyP& p, const PolicyLoad<T, KL, TA, N>& x, RowInfo row, float W, float* g, PolicyAcc& a) {
-  const float w = W * row.u, wk = w * p.kl_coef, fhi = p.fhi, flo = p.flo, fdual = p.fdual, vhi = p.vhi, vlo = p.vlo, vdual = p.vdual;
-  float reff = 0.f, kl = 0.f;
-  bool same = false;
-  unsigned cuts = 0;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const float A = TA ? x.a.at(k) : row.A;
-    const float border = A > 0.f ? fhi : (A < 0.f ? -flo : INFINITY), held = A > 0.f ? vhi : vlo;
-    const float l = x.l.at(k), d = l - (p.old ? x.o.at(k) : l);
-    const float sd = __uint_as_float(__float_as_uint(d) ^ (__float_as_uint(A) & 0x80000000u));
-    bool cut = sd > border;
-    same = same || sd == border;
-    const float rho = exp_near(d);
-    float r = cut ? held : rho, live = cut ? 0.f : rho;
-    if (DUAL) {
-      const bool far = A < 0.f && d > fdual;
-      same = same || d == fdual;
-      r = far ? vdual : r;
-      live = far ? 0.f : live;
-      cut = cut || far;
-    }
-    cuts += cut ? 1u : 0u;
-    a.rho += rho;
-    if (TA) {
-      reff = fmaf(-A, r, reff);
-      g[k] = -A * live * w;
-    } else {
-      reff += r;
-      g[k] = (-row.A * w) * live;
-    }
-    if (KL) {
-      float q, dk;
-      kl_term<KL>(x.f.at(k) - l, &q, &dk);
-      kl += q;
-      g[k] = fmaf(wk, dk, g[k]);
-    }
-  }
-  a.pg = row.u * (TA ? reff : -row.A * reff);
-  a.kl = row.u * kl;
-  a.cut = (1u << cuts) - 1u;                          // (as many bits as tokens beyond a border)
-  return !__any(same);
-}
-
-// Tokens [begin, end) of flat tensors by a workgroup.  (Loading a turn ahead was measured: 53 -> 68 us at 4096 x 8192 in
-// bfloat16, no gain in float32 -- the registers cost a wave on each SIMD.)
-template <typename T, int KL, bool TA, bool PACKED>
-__device__ __forceinline__ void policy_flat(const PolicyP& p, long long begin, long long end, float W, PolicySum& sum) {
-  constexpr int N = 16 / (int)sizeof(T);
-  const bool early = !p.tk.mask && !p.tk.lengths;     // nearly every token counts: its loads go out before what says so
-  Window win{-1, 0};
-  for (long long b = begin; b < end; b += 256 * N) {
-    const long long i = b + threadIdx.x * N, iw = uniform(b + (threadIdx.x & ~63) * N);
-    if (iw >= end) break;
-    const long long lw = iw + 64 * N <= end ? iw + 64 * N - 1 : end - 1;
-    const bool whole = i + N <= end;
-    PolicyLoad<T, KL, TA, N> x;
-    if (early && whole) x.load(p, i);
-    RowsOfPack q = PACKED ? rows_packed<N>(p, win, i, iw, lw) : rows_padded<N>(p, i, iw, lw);
-    if (!whole || q.single) {
-      const int m = whole ? N : (int)(end - i);
-      for (int k = 0; k < m; ++k) policy_one<T>(p, i + k, W, sum);
-      continue;
-    }
-    if (p.tk.mask) {
-      typedef unsigned char bytes __attribute__((ext_vector_type(N), aligned(1)));
-      const bytes m = *(const TREBI_GLOBAL bytes*)(p.tk.mask + i);
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (!m[k]) q.valid &= ~(1u << k);
-    }
-    if (!early && q.valid) x.load(p, i);
-    PolicyAcc a{0, 0, 0, 0};
-    float g[N];
-    bool done = __all(q.valid == low_bits(N)) && q.one_row;
-    if (done) {
-      done = p.fdual == INFINITY ? policy_row<T, KL, TA, N, false>(p, x, q.a, W, g, a) : policy_row<T, KL, TA, N, true>(p, x, q.a, W, g, a);
-      if (!done) a = PolicyAcc{0, 0, 0, 0};
-    }
-    if (done) {
-    } else if (q.valid) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const bool on = (q.valid >> k) & 1u, first = k < q.k1;
-        const float l = on ? x.l.at(k) : 0.f, o = on ? (p.old ? x.o.at(k) : l) : 0.f, f = KL && on ? x.f.at(k) : 0.f;
-        const float u = on ? (first ? q.a.u : q.b.u) : 0.f;
-        const float A = on ? (TA ? x.a.at(k) : (first ? q.a.A : q.b.A)) : 0.f;
-        const float d = policy_token<KL>(p, l, o, f, A, u, k, a);
-        g[k] = on ? W * u * d : 0.f;
-        if (!on) a.rho -= 1.f;                        // e^0
-      }
-      a.cut &= q.valid;
-    } else {
-#pragma unroll
-      for (int k = 0; k < N; ++k) g[k] = 0.f;
-    }
-    sum.pg += (double)a.pg;
-    if (KL) sum.kl += (double)a.kl;
-    sum.rho += (double)a.rho;
-    sum.cut += __popc(a.cut);
-    sum.cnt += __popc(q.valid);
-    if (p.grad) store_vec<N>((T*)p.grad + i, g);
-  }
-}
-
-__device__ __forceinline__ void policy_stats(const PolicyP& p, const double* v, double W) {
-  const double pg = W * v[0], kl = W * v[1], n = v[4] > 0.0 ? v[4] : 1.0;
-  p.stats[0] = (float)(pg + (double)p.kl_coef * kl);
-  p.stats[1] = (float)pg;
-  p.stats[2] = (float)kl;
-  p.stats[3] = (float)(v[2] / n);
-  p.stats[4] = (float)(v[3] / n);
-}
-
-// KIND 0: any strides, token by token; 1: flat padded rows; 2: packed
-template <typename T, int KL, bool TA, int KIND>
-__global__ __launch_bounds__(256) void policy_kernel(PolicyP p) {
-  __shared__ double lds[5 * LOSS_VALS];
-  const double W = policy_weight_parts<256>(p, lds);
-  const float Wg = (float)(W * (double)p.gscale);
-  const long long begin = (long long)blockIdx.x * p.per, end = begin + p.per < p.tk.n ? begin + p.per : p.tk.n;
-  PolicySum sum{0, 0, 0, 0, 0};
-  if (KIND == 0) {
-    for (long long i = begin + threadIdx.x; i < end; i += 256) policy_one<T>(p, i, Wg, sum);
-  } else {
-    policy_flat<T, KL, TA, KIND == 2>(p, begin, end, Wg, sum);
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0 && gridDim.x > 1) *p.weight = W;
-  double acc[LOSS_VALS] = {sum.pg, sum.kl, (double)sum.cut, sum.rho, (double)sum.cnt};
-  block_sum<LOSS_VALS, 256>(acc, lds);
-  if (threadIdx.x == 0) {
-    if (gridDim.x == 1) policy_stats(p, acc, W);
-    else
-#pragma unroll
-      for (int k = 0; k < LOSS_VALS; ++k) p.part[k * LOSS_PARTS + blockIdx.x] = acc[k];
-  }
-}
-
-__global__ __launch_bounds__(1024) void policy_finish_kernel(PolicyP p, int blocks) {
-  __shared__ double lds[17 * LOSS_VALS];
-  double v[LOSS_VALS] = {0, 0, 0, 0, 0};
-  for (int b = threadIdx.x; b < blocks; b += 1024)
-#pragma unroll
-    for (int k = 0; k < LOSS_VALS; ++k) v[k] += p.part[k * LOSS_PARTS + b];
-  block_sum<LOSS_VALS, 1024>(v, lds);
-  if (threadIdx.x == 0) policy_stats(p, v, blocks ? *p.weight : 0.0);
-}
-
 // Lanes a row is given: 16 bytes of mask each
 static int group_of(const TokenP& t) {
   const long long len = t.packed ? (t.n + t.rows - 1) / t.rows : t.len;
@@ -555,31 +88,23 @@ hipError_t launch_token_counts(const PolicyP& p, hipStream_t st) {
     hipLaunchKernelGGL(token_count_kernel, dim3(p.nnp), dim3(256), 0, st, t, group_of(t), p.np, p.counts);
   return hipGetLastError();
 }
-template <typename T, int KL>
-static hipError_t launch_policy_t(const PolicyP& p, int blocks, hipStream_t st) {
-#define GO(TA, KIND) hipLaunchKernelGGL((policy_kernel<T, KL, TA, KIND>), dim3(blocks), dim3(256), 0, st, p)
-  if (p.tk.packed) { if (p.acs) GO(true, 2); else GO(false, 2); }
-  else { if (p.acs) GO(true, 1); else GO(false, 1); }
-  return hipGetLastError();
-}
-template <typename T>
-static hipError_t launch_policy_k(const PolicyP& p, int blocks, hipStream_t st) {
-  if (!p.flat) {
-    hipLaunchKernelGGL((policy_kernel<T, 0, false, 0>), dim3(blocks), dim3(256), 0, st, p);
-    return hipGetLastError();
-  }
-  switch (p.ref ? p.kl : 0) {
-    case 0: return launch_policy_t<T, 0>(p, blocks, st);
-    case 1: return launch_policy_t<T, 1>(p, blocks, st);
-    case 2: return launch_policy_t<T, 2>(p, blocks, st);
-    default: return launch_policy_t<T, 3>(p, blocks, st);
-  }
-#undef GO
-}
+hipError_t launch_policy_f32(const PolicyP& p, int blocks, hipStream_t st);
+hipError_t launch_policy_bf16(const PolicyP& p, int blocks, hipStream_t st);
+hipError_t launch_policy_f16(const PolicyP& p, int blocks, hipStream_t st);
 hipError_t launch_policy(const PolicyP& p, int dtype, int blocks, hipStream_t st) {
-  return dtype == 0 ? launch_policy_k<float>(p, blocks, st) : dtype == 1 ? launch_policy_k<bf16_t>(p, blocks, st)
-                                                                         : launch_policy_k<f16_t>(p, blocks, st);
+  return dtype == 0 ? launch_policy_f32(p, blocks, st) : dtype == 1 ? launch_policy_bf16(p, blocks, st) : launch_policy_f16(p, blocks, st);
 }
+
+__global__ __launch_bounds__(1024) void policy_finish_kernel(PolicyP p, int blocks) {
+  __shared__ double lds[17 * LOSS_VALS];
+  double v[LOSS_VALS] = {0, 0, 0, 0, 0};
+  for (int b = threadIdx.x; b < blocks; b += 1024)
+#pragma unroll
+    for (int k = 0; k < LOSS_VALS; ++k) v[k] += p.part[k * LOSS_PARTS + b];
+  block_sum<LOSS_VALS, 1024>(v, lds);
+  if (threadIdx.x == 0) policy_stats(p, v, blocks ? *p.weight : 0.0);
+}
+
 hipError_t launch_policy_finish(const PolicyP& p, int blocks, hipStream_t st) {
   hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(1024), 0, st, p, blocks);
   return hipGetLastError();

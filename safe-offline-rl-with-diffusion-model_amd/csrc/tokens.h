@@ -166,4 +166,14 @@ __device__ __forceinline__ void row_bounds(const TokenP& t, long long r, long lo
   }
 }
 
+// The policy loss's scalars from its sums (pg, kl, cut, rho, count) and the weight
+__device__ __forceinline__ void policy_stats(const PolicyP& p, const double* v, double W) {
+  const double pg = W * v[0], kl = W * v[1], n = v[4] > 0.0 ? v[4] : 1.0;
+  p.stats[0] = (float)(pg + (double)p.kl_coef * kl);
+  p.stats[1] = (float)pg;
+  p.stats[2] = (float)kl;
+  p.stats[3] = (float)(v[2] / n);
+  p.stats[4] = (float)(v[3] / n);
+}
+
 }  // namespace trebi

@@ -158,14 +158,14 @@ def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, le
     stats = torch.empty(5, device=dev)
     lib = _lib.lib()
     ws_bytes = lib.trebi_policy_loss_workspace_bytes(d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     q = _POLICY.pack(
         _DTYPES[logp.dtype], logp.data_ptr(), 0 if logp_old is None else logp_old.data_ptr(),
         0 if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1], *strides[2], advantages.data_ptr(),
         *adv_stride, 0 if grad is None else grad.data_ptr(), stats.data_ptr(), clip, clip if clip_high is None else clip_high,
         0.0 if dual_clip is None else dual_clip, kl_coef, _KL[kl], _REDUCTIONS[reduction] if denominator is None else 2,
         0.0 if denominator is None else denominator, grad_scale)
-    rc = lib.trebi_policy_loss(_lib.ctx(dev.index or 0), d, q, ws.data_ptr(), ws_bytes, _lib.stream(dev))
+    rc = lib.trebi_policy_loss(_lib.ctx(dev.index or 0), d, q, None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream(dev))
     if rc:
         _lib.check(rc)
     loss, policy, klv, cut, ratio = stats.unbind()
@@ -223,13 +223,13 @@ def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=
     out = torch.empty(2 * P + 3, device=dev)
     lib = _lib.lib()
     ws_bytes = lib.trebi_preference_loss_workspace_bytes(d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     at = out.data_ptr()
     q = _PREFERENCE.pack(
         _DTYPES[logp.dtype], logp.data_ptr(), 0 if logp_ref is None else logp_ref.data_ptr(), *strides[0], *strides[1],
         0 if weights is None else weights.data_ptr(), 0 if grad is None else grad.data_ptr(), at, at + 4 * P, at + 8 * P, beta,
         label_smoothing, margin, _KINDS[kind], int(bool(average)), 0.0 if denominator is None else denominator, grad_scale)
-    rc = lib.trebi_preference_loss(_lib.ctx(dev.index or 0), d, q, ws.data_ptr(), ws_bytes, _lib.stream(dev))
+    rc = lib.trebi_preference_loss(_lib.ctx(dev.index or 0), d, q, None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream(dev))
     if rc:
         _lib.check(rc)
     chosen, rejected, stats = out.split((P, P, 3))

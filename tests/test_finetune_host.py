@@ -61,9 +61,11 @@ def test_token_descriptions_refused(change, code, word):
 
 def test_policy_loss_workspace_and_strides():
     lib = _lib.lib()
-    d = tokens()
+    assert lib.trebi_policy_loss_workspace_bytes(C.byref(tokens())) == 0      # one workgroup does it all
+    d = tokens(len=100000)
     need = lib.trebi_policy_loss_workspace_bytes(C.byref(d))
     assert 0 < need < 1 << 20
+    refused(lib.trebi_policy_loss(CTX, C.byref(d), C.byref(policy()), None, need, None), -1, 'null')
     refused(lib.trebi_policy_loss(CTX, C.byref(d), C.byref(policy()), PTR, need - 1, None), -4, 'workspace')
     masked = tokens(mask=PTR, rows=1000000)
     assert lib.trebi_policy_loss_workspace_bytes(C.byref(masked)) >= need + 4000000
@@ -88,6 +90,8 @@ def test_preference_loss_refuses_odd_rows_and_small_workspaces():
     d = tokens(rows=48, len=100000)
     need = lib.trebi_preference_loss_workspace_bytes(C.byref(d))
     refused(lib.trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), PTR, need - 1, None), -4, 'workspace')
+    refused(lib.trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), None, need, None), -1, 'workspace')
+    assert lib.trebi_preference_loss_workspace_bytes(C.byref(tokens())) == 0
 
 
 def transition(**kw):
