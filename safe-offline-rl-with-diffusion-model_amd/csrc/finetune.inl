@@ -224,6 +224,8 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
   if (d->reduction < 0 || d->reduction > 2) return fail(TREBI_BAD_ARG, "reduction must be 0 (token), 1 (sequence) or 2 (denominator)");
   if (!(d->clip_low >= 0.f) || !(d->clip_high >= 0.f)) return fail(TREBI_BAD_ARG, "clip ranges must not be negative");
   if (d->dual_clip != 0.f && !(d->dual_clip > 1.f)) return fail(TREBI_BAD_ARG, "dual_clip must be above 1 (or 0: off)");
+  if (d->reduction == 1 && tokens->mask && tokens->len > 0x7fffffff)
+    return fail(TREBI_UNSUPPORTED_CONFIG, "the mean over masked sequences counts at most 2^31 - 1 tokens a row");
   if (d->reduction == 2 && !(d->denominator > 0.0)) return fail(TREBI_BAD_ARG, "denominator must be positive");
   if (workspace_bytes < policy_bytes(*tokens)) return fail(TREBI_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, policy_bytes(*tokens));
   p.lp = d->logp; p.old = d->logp_old; p.ref = d->logp_ref;

@@ -401,7 +401,8 @@ __device__ __forceinline__ void policy_pack(const PolicyP& p, const Window& w, l
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       for (;;) {                                      // past the sequences that end here (empty ones too)
-        const bool on = pos < 62 && w.r + pos + 1 < p.tk.rows && (long long)__shfl(w.at, pos + 1, 64) <= i + k;
+        const long long next = __shfl(w.at, pos + 1, 64);                // (by all lanes: a lane that sat out could not be read)
+        const bool on = pos < 62 && w.r + pos + 1 < p.tk.rows && next <= i + k;
         if (!__any(on)) break;
         pos += on;
       }

@@ -56,6 +56,7 @@ class GradClipper:
         self.set = _lib.GradSet()
         _lib.check(lib.trebi_grad_set_fill(n, ptrs, numels, dtypes, _lib.ptr(host), nbytes, C.byref(self.set)))
         self.table = host.to(self.device)
+        self._spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.tensors]
         self.total = int(self.set.total)
         self._ws_bytes = lib.trebi_grad_workspace_bytes(C.byref(self.set))
         self._fixed = (_lib.ctx(self.device.index or 0), C.byref(self.set), C.c_void_p(self.table.data_ptr()), self.norm_type)
@@ -86,8 +87,8 @@ class GradClipper:
             raise RuntimeError(f'out must be a contiguous float32 [{self.total}] on {self.device}')
         else:
             lo, hi = out.data_ptr(), out.data_ptr() + 4 * self.total
-            for i, t in enumerate(self.tensors):
-                if t.data_ptr() < hi and lo < t.data_ptr() + t.numel() * t.element_size():
+            for i, (a, b) in enumerate(self._spans):
+                if a < hi and lo < b:
                     raise RuntimeError(f'out overlaps tensor {i}; use clip_ to scale in place')
         ws, norm, st = self._buffers()
         _lib.check(_lib.lib().trebi_grad_clip(*self._fixed, max_norm, grad_scale, out.data_ptr() or ws.data_ptr(),

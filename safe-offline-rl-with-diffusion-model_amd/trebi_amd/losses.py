@@ -63,6 +63,8 @@ def _ints(name, v, n, device):
         v = torch.as_tensor(v)
     if v.shape != (n,) and n is not None or v.dim() != 1 or v.is_floating_point() or v.dtype == torch.bool:
         raise ValueError(f'{name} must be an integer tensor of shape [{n if n is not None else "rows + 1"}], got {v.dtype} {tuple(v.shape)}')
+    if v.dtype is torch.int64:
+        v = v.clamp(-1, 2 ** 31 - 1)                                # cut to the tensor later, but not wrapped around before
     return v.to(device, torch.int32).contiguous()
 
 

@@ -59,6 +59,11 @@ def test_token_descriptions_refused(change, code, word):
     refused(_lib.lib().trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), PTR, 1 << 40, None), code, word)
 
 
+def test_policy_loss_refuses_masked_rows_beyond_32_bits():
+    d, q = tokens(rows=1, len=1 << 31, mask=PTR), policy(reduction=1)
+    refused(_lib.lib().trebi_policy_loss(CTX, C.byref(d), C.byref(q), PTR, 1 << 40, None), -3, 'masked')
+
+
 def test_policy_loss_workspace_and_strides():
     lib = _lib.lib()
     assert lib.trebi_policy_loss_workspace_bytes(C.byref(tokens())) == 0      # one workgroup does it all

@@ -159,6 +159,82 @@ def test_policy_loss_reads_views(strided, dtype):
         run_policy('packed', 9, 21, dtype, strided=strided, kl_coef=0.1)
 
 
+def packed_case(lens, front, tail, seed, dtype, masked=False, adv='row', **kw):
+    """A packed policy loss with the given sequence lengths against its definition."""
+    from trebi_amd.losses import policy_loss
+    g = torch.Generator().manual_seed(seed)
+    cu = np.concatenate([[0], np.cumsum(lens)]) + front
+    n = int(cu[-1]) + tail
+    base = -torch.rand(n, generator=g) * 3
+    logp, old, ref = ((base + torch.randn(n, generator=g) * s).to(DT[dtype]) for s in (0.0, 0.3, 0.5))
+    m = np.random.default_rng(seed).random(n) < 0.7 if masked else np.ones(n, bool)
+    picks = [np.arange(cu[r], cu[r + 1])[m[cu[r]:cu[r + 1]]] for r in range(len(lens))]
+    A = torch.randn(*((len(lens),) if adv == 'row' else (n,)), generator=g)
+    which = dict(cu_seqlens=torch.tensor(cu, dtype=torch.int64).cuda())
+    if masked:
+        which['mask'] = torch.from_numpy(m).cuda()
+    r = policy_loss(logp.cuda(), A.cuda(), old.cuda(), ref.cuda(), per_token=adv == 'token', **which, **kw)
+    Ar = [np.full(len(p), np64(A)[i]) if adv == 'row' else np64(A)[p] for i, p in enumerate(picks)]
+    want = F.policy(rows_of(logp, picks), Ar, rows_of(old, picks), rows_of(ref, picks), coef=kw.get('kl_coef', 0.0),
+                    kl=kw.get('kl', 'k3'), reduction=kw.get('reduction', 'token'), dual=kw.get('dual_clip'))
+    check_policy(r, want, picks, dtype, dict(abs_pg=float(A.abs().max()) * 5, abs_kl=20), (len(lens), front, tail, dtype))
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+@pytest.mark.parametrize('masked', [False, True])
+def test_policy_loss_packed_clusters(dtype, masked):
+    """Runs of tiny and empty sequences between long ones: several in one thread's tokens, more than a wave looks at together."""
+    rng = np.random.default_rng(5)
+    tiny = lambda k: list(rng.integers(0, 4, size=k))
+    for n, lens in enumerate([tiny(40) + [3000] + tiny(30), [5000] + tiny(300) + [1] * 50 + [4000], [0] * 200 + [2500] + [0] * 200,
+                              [2, 9, 1, 0, 0, 7, 3, 1, 1, 1, 2048, 1, 2, 3, 4, 5, 6, 7, 8, 700], [1] * 3 + [4096] + [1] * 3, [6000],
+                              [0, 0, 0, 6001, 0], tiny(900) + [9000]]):
+        for reduction in ('token', 'sequence'):
+            packed_case(lens, front=n % 3, tail=n % 5, seed=n, dtype=dtype, masked=masked, adv='token' if n % 2 else 'row',
+                        reduction=reduction, kl_coef=0.1, kl=('k1', 'k2', 'k3')[n % 3], dual_clip=3.0 if n % 4 == 0 else None)
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+def test_policy_loss_every_tail(dtype):
+    """Token counts one by one around a thread's, a wave's and a workgroup's share, in one workgroup and in several."""
+    for n in list(range(1, 20)) + [255, 257, 511, 513, 1023, 1025, 2047, 2049, 4095, 4096, 4097, 4099, 8191, 8193, 20479, 20487]:
+        packed_case([n - n // 3, n // 3], 0, 0, n, dtype)
+    for L in (511, 513, 4095, 4096, 4097, 4100, 10241):
+        run_policy('all', 1, L, dtype, seed=L)
+        run_policy('mask', 3, L, dtype, seed=L)
+
+
+def test_masks_of_other_types_and_shapes():
+    from trebi_amd.losses import policy_loss, preference_loss
+    g = torch.Generator('cuda').manual_seed(0)
+    lp, old = (-torch.rand(6, 300, device='cuda', generator=g) for _ in range(2))
+    adv = torch.randn(6, device='cuda', generator=g)
+    m = torch.rand(6, 300, device='cuda', generator=g) < 0.5
+    for other in (m.to(torch.uint8) * 7, m.float(), m.long(), m.t().contiguous().t()):
+        a, b = policy_loss(lp, adv, old, mask=m), policy_loss(lp, adv, old, mask=other)
+        assert torch.equal(a.grad, b.grad) and abs(float(a.loss) - float(b.loss)) <= 2 * ULP * float(adv.abs().max()) * 3
+        p, q = preference_loss(lp, old, mask=m), preference_loss(lp, old, mask=other)
+        assert torch.equal(p.grad, q.grad) and torch.equal(p.chosen_reward, q.chosen_reward)
+    one = m[:1].expand(6, 300)                              # a mask that all rows share
+    a, b = policy_loss(lp, adv, old, mask=one, reduction='sequence'), policy_loss(lp, adv, old, mask=one.contiguous(), reduction='sequence')
+    assert not a.grad[~one].any() and (a.grad - b.grad).abs().max() <= 2 * ULP * float(adv.abs().max()) / 100
+    shared = lp[:1].expand(6, 300)                          # log-probabilities that all rows share: a gradient for each
+    assert policy_loss(shared, adv, shared - 0.1).grad.shape == (6, 300)
+    a, b = policy_loss(lp, adv[:, None].expand(6, 300), old), policy_loss(lp, adv, old)
+    assert torch.equal(a.grad, b.grad)
+
+
+def test_offsets_of_64_bits_do_not_wrap():
+    from trebi_amd.losses import policy_loss
+    lp = -torch.rand(36, device='cuda')
+    adv = torch.ones(2, device='cuda')
+    a = policy_loss(lp, adv, cu_seqlens=torch.tensor([0, 7, 2 ** 32 + 3], device='cuda'))
+    b = policy_loss(lp, adv, cu_seqlens=torch.tensor([0, 7, 36], device='cuda'))
+    assert torch.equal(a.grad, b.grad) and a.grad.all()
+    a = policy_loss(lp.view(2, 18), adv, lengths=torch.tensor([5, 2 ** 32], device='cuda'))
+    assert a.grad[1].all() and not a.grad[0, 5:].any()
+
+
 def test_policy_loss_without_old_or_reference_and_with_a_denominator():
     run_policy('lengths', 6, 30, 'float32', has_old=False, has_ref=False)
     run_policy('packed', 6, 30, 'bfloat16', has_old=False, kl_coef=0.2)
