@@ -16,6 +16,7 @@ struct GradP {
   const GradChunk* chunks;
   int n_chunks, n_blocks, norm_type;       // 0 two-norm, 1 one-norm, 2 largest magnitude
   int stream_loads, stream_stores;         // past the caches: nothing will read it from there
+  int one_each;                            // one chunk of at most 4096 elements for each workgroup
   float grad_scale, max_norm;
   float* out;                              // flat float32 copy, or null: in place
   float* norm_out;                         // [1] or null

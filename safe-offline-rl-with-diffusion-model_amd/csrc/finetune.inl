@@ -62,6 +62,7 @@ int grad_args(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int 
   p->n_chunks = set->n_chunks;
   const int rounds = std::max(1, (set->n_chunks + GRAD_BLOCKS - 1) / GRAD_BLOCKS);    // the same number of chunks for every workgroup
   p->n_blocks = std::max(1, (set->n_chunks + rounds - 1) / rounds);
+  p->one_each = set->n_chunks > 0 && set->n_chunks <= GRAD_BLOCKS && grad_chunk(set->total) <= 4096;
   p->norm_type = norm_type;
   p->grad_scale = grad_scale;
   p->part = (double*)ws;

@@ -11,6 +11,8 @@
 #include "finetune.h"
 #include "tokens.h"
 
+#include <type_traits>
+
 namespace trebi {
 
 template <int NORM>
@@ -196,6 +198,52 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(GradP p) {
   }
 }
 
+// The same for sets of one chunk a workgroup (a few million elements), which latency bounds: the chunk's loads are on their
+// way while the partial sums are added up.
+__global__ __launch_bounds__(256) void grad_scale_small_kernel(GradP p) {
+  __shared__ double lds[4];
+  typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
+  const GradChunk t = uniform_load(p.chunks + blockIdx.x);
+  const int V = t.dtype == 0 ? 4 : 8, whole = t.len & ~(V - 1), size = t.dtype == 0 ? 4 : 2;
+  u4 r[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int i = (u * 256 + (int)threadIdx.x) * V;
+    if (i < whole) r[u] = *(const TREBI_GLOBAL u4*)((const char*)t.p + (size_t)i * size);
+  }
+  float c;
+  const float norm = grad_total<256>(p, lds, &c);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.norm_out) *p.norm_out = norm;
+  if (!p.out && c == 1.f) return;
+  float* o = p.out ? p.out + t.out_off : nullptr;
+  auto put = [&](auto* src, auto* dst) {
+    typedef typename std::remove_pointer<decltype(src)>::type T;
+    constexpr int W = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = (u * 256 + (int)threadIdx.x) * W;
+      if (i < whole) {
+        union { u4 q; typename Raw<T>::type e[W]; } x;
+        x.q = r[u];
+        float v[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] = up(x.e[k]) * c;
+        store_vec<W>(dst + i, v);
+      }
+    }
+    const int i = whole + (int)threadIdx.x;
+    if (i < t.len) store_one(dst + i, load_one(src + i) * c);
+  };
+  if (t.dtype == 0) put((float*)t.p, o ? o : (float*)t.p);
+  else if (t.dtype == 1) {
+    if (o) put((bf16_t*)t.p, o);
+    else put((bf16_t*)t.p, (bf16_t*)t.p);
+  } else {
+    if (o) put((f16_t*)t.p, o);
+    else put((f16_t*)t.p, (f16_t*)t.p);
+  }
+}
+
 hipError_t launch_grad_partials(const GradP& p, hipStream_t st) {
   const dim3 g(p.n_blocks), b(256);
 #define GO(N)                                                                                  \
@@ -214,7 +262,8 @@ hipError_t launch_grad_finish(const GradP& p, float* coef_out, hipStream_t st) {
   return hipGetLastError();
 }
 hipError_t launch_grad_scale(const GradP& p, hipStream_t st) {
-  if (p.stream_stores) hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(p.n_blocks), dim3(256), 0, st, p);
+  if (p.one_each) hipLaunchKernelGGL(grad_scale_small_kernel, dim3(p.n_blocks), dim3(256), 0, st, p);
+  else if (p.stream_stores) hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(p.n_blocks), dim3(256), 0, st, p);
   else hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(p.n_blocks), dim3(256), 0, st, p);
   return hipGetLastError();
 }

@@ -275,7 +275,9 @@ def _transition(model, pred, x, x_prev, t, cond_keys):
         raise ValueError(f't must be [{B}] integers, got {t.dtype} {tuple(t.shape)}')
     if not t.is_cuda and B and not (0 <= int(t.min()) and int(t.max()) < T):
         raise RuntimeError(f'timesteps must lie in [0, {T})')
-    t = t.to(dev, torch.int64).contiguous()
+    if t.dtype is not torch.int64 or t.device != dev:
+        t = t.to(dev, torch.int64)
+    t = t.contiguous()
     keys = sorted(int(k) for k in cond_keys)
     if len(keys) > 4:
         raise RuntimeError('at most 4 conditioned timesteps are supported')
