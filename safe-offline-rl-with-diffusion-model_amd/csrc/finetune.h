@@ -79,14 +79,14 @@ struct PairP {
   float smooth, gscale;
   int kind, average;                       // 0 sigmoid, 1 hinge, 2 ipo
   float *rew_c, *rew_r;                    // [pairs]
-  double* part;                            // [blocks or pairs][4]: loss, hits, z, pairs that count
-  int nparts;
+  double* part;                            // [nparts][4]: loss, hits, z, pairs that count
+  int nparts;                              // workgroups, or pairs where rows are split
   float* stats;                            // [3]
   int group;                               // threads of a pair (whole-pair kernel)
   int splits;                              // workgroups of a row (split kernels)
   double* rowpart;                         // [rows][splits][2]: sum, count
 };
-hipError_t launch_pairs_whole(const PairP& p, int dtype, int blocks, hipStream_t st);
+hipError_t launch_pairs_whole(const PairP& p, int dtype, hipStream_t st);     // of p.nparts workgroups
 hipError_t launch_pairs_split(const PairP& p, int dtype, hipStream_t st);
 hipError_t launch_pairs_finish(const PairP& p, hipStream_t st);
 

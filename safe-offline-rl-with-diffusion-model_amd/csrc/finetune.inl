@@ -24,12 +24,14 @@ struct DeviceGuard {
 
 size_t al256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Elements of a chunk: whole turns of a workgroup (256 threads x 8 loads of 16 bytes: 16384 16-bit or 8192 32-bit elements),
-// about 8 chunks a workgroup of a large set; smaller sets are cut finer, so that they reach every CU.
+// Elements of a chunk.  Up to 8 M elements each workgroup gets one of 4096, whose loads are all in flight at once (bfloat16,
+// 4 M elements in 50 tensors, clipped in place: 9.2 us, with 16384 13.2; 2 M: 7.2, with 2048 8.2).  Larger sets: whole turns of a
+// workgroup (256 threads x 8 loads of 16 bytes: 16384 16-bit or 8192 32-bit elements), at most about 8 chunks each, so that
+// all end together (20 M: 24 us, with 4096 29; 400 M: 442, with 4096 461).
 long long grad_chunk(long long total) {
+  if (total <= 4096ll * GRAD_BLOCKS) return 4096;
   const long long per = (total + 8 * GRAD_BLOCKS - 1) / (8 * GRAD_BLOCKS);
-  if (per > 4096) return std::min<long long>((per + 16383) / 16384 * 16384, 1 << 28);
-  return total > 2048 * 1024 ? 4096 : 2048;
+  return std::min<long long>((per + 16383) / 16384 * 16384, 1 << 28);
 }
 
 int grad_totals(int n, const int64_t* numels, long long* total, long long* chunks) {
@@ -47,7 +49,8 @@ int grad_totals(int n, const int64_t* numels, long long* total, long long* chunk
 }
 
 // From this many bytes on the 256 MB cache cannot hand a set from one kernel to the next: such sets are read (for the norm
-// alone) and written past the caches.
+// alone) and written past the caches.  Norm of 366 MB 59 us, through them 67; 976 MB 151 and 172; 244 MB: 42 both ways.
+// Clipping 800 MB of bfloat16 in place: 315 us, through them 353.
 constexpr long long GRAD_STREAM = 256ll << 20;
 
 int grad_args(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float grad_scale, void* ws,
@@ -93,8 +96,13 @@ int token_args(const trebi_token_desc& d, TokenP* t) {
   return 0;
 }
 
+// One workgroup does it all up to 4096 tokens (at most 4 turns): calls of this size wait for their launches.  4096 float32 tokens
+// with lengths, enqueued one by one: 14 us, with three launches 20 (replayed from a graph 10.5 and 10.4); 8192, replayed: 17.5 and 10.8.
 // policy workspace: partial counts, partial sums, a count for each row; a call of one workgroup without a mask needs none
 constexpr long long SINGLE = 4096;
+// Up to this many rows every workgroup adds their lengths up for itself, which saves a launch: 1024 x 1024 float32 with lengths
+// 12.7 us against 14.5, 2048 x 1024 16.3 and 17.2, 4096 x 1024 24.7 and 22.5, 16384 x 1024 71 and 53.
+constexpr long long COUNT_ROWS = 2048;
 size_t policy_bytes(const trebi_token_desc& d) {
   if (!d.mask && d.rows >= 0 && d.rows <= SINGLE && d.len >= 0 && (d.packed || d.len <= SINGLE) && (d.packed ? d.len : d.rows * d.len) <= SINGLE) return 0;
   return al256(COUNT_BLOCKS * sizeof(NormPart)) + al256((LOSS_PARTS * LOSS_VALS + 1) * sizeof(double)) +
@@ -102,28 +110,33 @@ size_t policy_bytes(const trebi_token_desc& d) {
 }
 
 constexpr int PAIR_BLOCKS = 2048;
-// Rows are split over workgroups where whole pairs would leave the card idle: fewer pairs than 2 a CU, and rows of
-// more than one turn of a workgroup.  (Lengths on the device do not matter for the choice, nor for the result.)
+// Rows are split over workgroups where whole pairs would leave the card idle: at most one pair a CU, and rows long enough to
+// pay for the second read and the third launch.  float32: 24 pairs of 131072 tokens 22 us, whole 80; 24 x 16384 10 and 15; 100 x
+// 16384 17 both ways; 250 x 16384 25, whole 22; 24 x 8192 10 both ways.  (Lengths on the device do not matter for the choice.)
 int pair_splits(const trebi_token_desc& d) {
   const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len;
-  if (d.rows / 2 >= 512 || len <= 4096) return 0;
+  if (d.rows > 512 || len <= 8192 || len < 64 * d.rows) return 0;
   return (int)std::max<long long>(1, std::min<long long>(PAIR_BLOCKS / d.rows, (len + 4095) / 4096));
 }
-// Threads of a pair: at most two turns of 16 tokens each, on average
+// Threads of a pair.  A wave pays for its pairs' scalars (a few hundred instructions) whatever it holds: few pairs take a whole
+// workgroup each, many pairs of short rows 16 threads.  bfloat16, us with 16 / 64 / 256 threads: 512 pairs of 60 tokens 7.5 / 7.7 /
+// 7.7, of 500 10.7 / 8.0 / 7.6, of 2000 25 / 12 / 8.5; 2000 of 1000 17 / 12 / 15; 8000 of 200 11 / 17 / 33.
 int pair_group(const trebi_token_desc& d) {
-  const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len;
-  return len <= 128 ? 16 : len <= 512 ? 64 : 256;
+  const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len, pairs = d.rows / 2;
+  if (len <= 128 || (pairs > 4096 && len <= 512)) return 16;
+  return pairs > 1024 && len <= 4096 ? 64 : 256;
 }
-int pair_blocks(const trebi_token_desc& d) {
-  const int g = pair_group(d), per = 256 / g;
-  return (int)std::min<long long>(PAIR_BLOCKS, (d.rows / 2 + per - 1) / per);
+long long pair_blocks(const trebi_token_desc& d) {
+  const int per = 256 / pair_group(d);
+  return (d.rows / 2 + per - 1) / per;
 }
 // preference workspace: partial sums, the rows' parts; a call of one workgroup needs none
 size_t pair_bytes(const trebi_token_desc& d) {
   if (d.rows < 2) return 0;
   const int s = pair_splits(d);
   if (!s && pair_blocks(d) == 1) return 0;
-  return al256(PAIR_BLOCKS * 4 * sizeof(double)) + (s ? al256((size_t)d.rows * s * 2 * sizeof(double)) : 0);
+  return s ? al256((size_t)d.rows / 2 * 4 * sizeof(double)) + al256((size_t)d.rows * s * 2 * sizeof(double))
+           : al256((size_t)pair_blocks(d) * 4 * sizeof(double));
 }
 
 }  // namespace
@@ -275,16 +288,15 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
   p.counts = t.mask && p.mode == 1 ? (int*)w : nullptr;
   hipStream_t st = (hipStream_t)stream;
   ON_DEVICE(ctx);
-  // One workgroup does it all up to 4096 tokens (at most 4 turns): a call of this size is bound by its launches.
   const long long turn = 256 * pack, turns = (t.n + turn - 1) / turn;
-  // ... else as many workgroups as fit on the 256 CUs at once, so that none is left for a second round: 5 or (see the kernel) 4
+  // as many workgroups as fit on the 256 CUs at once, so that none is left for a second round: 5 or (see the kernel) 4
   const long long most = t.packed || p.acs || (p.ref && p.kl == 3) ? 1024 : LOSS_PARTS;
   const long long per = t.n <= SINGLE ? std::max<long long>(turns, 1) : (turns + most - 1) / most;
   const int blocks = (int)((turns + per - 1) / per);
   p.per = per * turn;
   p.early = all || (t.packed && !t.mask) || per == 1;
   const bool told = t.packed && p.mode == 0 && !t.mask;               // the offsets say how many tokens there are
-  if (!empty && !told && (p.counts || (p.fixed == 0.0 && (blocks > 1 || t.mask || t.rows > SINGLE)))) {
+  if (!empty && !told && (p.counts || (p.fixed == 0.0 && (t.mask || t.rows > (blocks == 1 ? SINGLE : COUNT_ROWS))))) {
     p.nnp = (int)(t.mask ? std::min<long long>(COUNT_BLOCKS, t.rows) : std::min<long long>(COUNT_BLOCKS, (t.rows + 255) / 256));
     HIPCHK(launch_token_counts(p, st));
   }
@@ -305,6 +317,7 @@ extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tok
   PairP p{};
   if (int e = token_args(*tokens, &p.tk)) return e;
   if (p.tk.rows < 2 || p.tk.rows % 2) return fail(TREBI_BAD_SHAPE, "%lld rows: chosen and rejected rows come in pairs", (long long)p.tk.rows);
+  if (!pair_splits(*tokens) && pair_blocks(*tokens) > 0xffffff) return fail(TREBI_UNSUPPORTED_CONFIG, "too many pairs for one call");
   if (!d->stats || !d->chosen_reward || !d->rejected_reward || (p.tk.n > 0 && !d->logp)) return fail(TREBI_BAD_ARG, "null argument");
   if (d->dtype < 0 || d->dtype > 2) return fail(TREBI_BAD_ARG, "unknown type %d", d->dtype);
   if (d->kind < 0 || d->kind > 2) return fail(TREBI_BAD_ARG, "kind must be 0 (sigmoid), 1 (hinge) or 2 (ipo)");
@@ -326,8 +339,8 @@ extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tok
   p.rew_c = d->chosen_reward; p.rew_r = d->rejected_reward;
   p.stats = d->stats;
   p.part = (double*)workspace;
-  p.rowpart = (double*)((char*)workspace + al256(PAIR_BLOCKS * 4 * sizeof(double)));
   p.splits = pair_splits(*tokens);
+  p.rowpart = !p.splits ? nullptr : (double*)((char*)workspace + al256((size_t)p.pairs * 4 * sizeof(double)));
   hipStream_t st = (hipStream_t)stream;
   ON_DEVICE(ctx);
   if (p.splits) {
@@ -335,9 +348,8 @@ extern "C" int trebi_preference_loss(trebi_ctx* ctx, const trebi_token_desc* tok
     HIPCHK(launch_pairs_split(p, d->dtype, st));
   } else {
     p.group = pair_group(*tokens);
-    const int blocks = pair_blocks(*tokens);
-    p.nparts = blocks;
-    HIPCHK(launch_pairs_whole(p, d->dtype, blocks, st));
+    p.nparts = (int)pair_blocks(*tokens);
+    HIPCHK(launch_pairs_whole(p, d->dtype, st));
   }
   if (p.splits || p.nparts > 1) HIPCHK(launch_pairs_finish(p, st));
   return 0;

@@ -80,6 +80,7 @@ __device__ __forceinline__ unsigned mask_bits(const TokenP& t, long long off, lo
 }
 
 // Sum and number of a row's valid tokens in [s, e), by `G` threads; this thread's part.  16 tokens a thread on their way.
+// Differences are taken in float64, where they are exact.
 template <typename T>
 __device__ __forceinline__ void pair_row_sum(const PairP& p, long long r, long long s, long long e, int lane, int G, double* sum,
                                              long long* num) {
@@ -107,22 +108,22 @@ __device__ __forceinline__ void pair_row_sum(const PairP& p, long long r, long l
         c += __popc(v[h]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const double d = ref ? (double)x[h].at(k) - (double)y[h].at(k) : (double)x[h].at(k);
-          a += (v[h] >> k) & 1u ? d : 0.0;
+          const bool on = (v[h] >> k) & 1u;
+          a += (double)(on ? x[h].at(k) : 0.f) - (double)(on && ref ? y[h].at(k) : 0.f);
         }
       }
     }
     // the last tokens, fewer than 8: one a lane
     const long long i = s + (e > s ? (e - s) / 8 * 8 : 0) + lane;
     if (lane < 8 && i < e && (!t.mask || t.mask[mb + i * t.mcs])) {
-      a += ref ? (double)load_one(lp + i) - (double)load_one(ref + i) : (double)load_one(lp + i);
+      a += (double)load_one(lp + i) - (ref ? (double)load_one(ref + i) : 0.0);
       ++c;
     }
   } else {
     for (long long i = s + lane; i < e; i += G) {
       if (t.mask && !t.mask[mb + i * t.mcs]) continue;
       const float x = load_one(lp + i * p.lcs);
-      a += ref ? (double)x - (double)load_one(ref + i * p.rcs) : (double)x;
+      a += (double)x - (ref ? (double)load_one(ref + i * p.rcs) : 0.0);
       ++c;
     }
   }
@@ -163,63 +164,62 @@ __device__ __forceinline__ void pair_gaps(const PairP& p) {
 }
 
 // G threads take a pair, half of them a row: the rows' sums, the pair, the rows' gradients.  Where there are pairs enough
-// to fill the card this is one pass: the gradient needs no second read of the log-probabilities.
-template <typename T>
-__global__ __launch_bounds__(256) void pairs_whole_kernel(PairP p) {
+// to fill the card this is one pass: the gradient needs no second read of the log-probabilities.  A workgroup takes 256 / G
+// pairs and ends: in a loop over pairs the compiler kept what does not change in registers, 190 of them.
+template <typename T, int G>
+__global__ __launch_bounds__(256, 4) void pairs_whole_kernel(PairP p) {
   __shared__ double lds[20];
-  const int G = p.group, half = G >> 1, per = 256 / G, gi = threadIdx.x / G, lane = threadIdx.x & (half - 1);
+  constexpr int half = G >> 1, per = 256 / G;
+  const int gi = threadIdx.x / G, lane = threadIdx.x & (half - 1);
   const bool second = threadIdx.x & half;
-  double acc[4] = {0, 0, 0, 0};
-  for (long long k0 = (long long)blockIdx.x * per; k0 < p.pairs; k0 += (long long)gridDim.x * per) {
-    const long long k = k0 + gi, r = second ? k + p.pairs : k;
-    const bool on = k < p.pairs;
-    long long s = 0, e = 0, n = 0;
-    double v[2] = {0, 0}, o[2];
-    if (on) {
-      row_bounds(p.tk, r, &s, &e);
-      pair_row_sum<T>(p, r, s, e, lane, half, &v[0], &n);
-      v[1] = (double)n;
-    }
-    if (G <= 64) {
-      for (int q = half >> 1; q > 0; q >>= 1) {
-        v[0] += __shfl_xor(v[0], q, 64);
-        v[1] += __shfl_xor(v[1], q, 64);
-      }
-      o[0] = __shfl_xor(v[0], half, 64);
-      o[1] = __shfl_xor(v[1], half, 64);
-    } else {                                          // the workgroup takes one pair, half of its waves a row
-      constexpr int HW = 2;
-      __syncthreads();
-      v[0] = wave_sum64(v[0]);
-      v[1] = wave_sum64(v[1]);
-      if ((threadIdx.x & 63) == 0) {
-        lds[(threadIdx.x >> 6) * 2] = v[0];
-        lds[(threadIdx.x >> 6) * 2 + 1] = v[1];
-      }
-      __syncthreads();
-      const int mine = second ? 2 * HW : 0, other = 2 * HW - mine;
-      v[0] = v[1] = o[0] = o[1] = 0.0;
+  const long long k = (long long)blockIdx.x * per + gi, r = second ? k + p.pairs : k;
+  const bool on = k < p.pairs;
+  double acc[4] = {0, 0, 0, 0}, v[2] = {0, 0}, o[2];
+  long long s = 0, e = 0, n = 0;
+  if (on) {
+    row_bounds(p.tk, r, &s, &e);
+    pair_row_sum<T>(p, r, s, e, lane, half, &v[0], &n);
+    v[1] = (double)n;
+  }
+  if (G <= 64) {
 #pragma unroll
-      for (int w = 0; w < HW; ++w) {
-        v[0] += lds[mine + 2 * w];
-        v[1] += lds[mine + 2 * w + 1];
-        o[0] += lds[other + 2 * w];
-        o[1] += lds[other + 2 * w + 1];
-      }
+    for (int q = half >> 1; q > 0; q >>= 1) {
+      v[0] += __shfl_xor(v[0], q, 64);
+      v[1] += __shfl_xor(v[1], q, 64);
     }
-    if (on) {
-      float rc, rr;
-      const PairOut q = pair_math(p, k, second ? o[0] : v[0], second ? o[1] : v[1], second ? v[0] : o[0], second ? v[1] : o[1], &rc, &rr);
-      if (lane == 0 && !second) {
-        p.rew_c[k] = rc;
-        p.rew_r[k] = rr;
-        acc[0] += q.loss; acc[1] += q.hit; acc[2] += q.z; acc[3] += q.on;
-      }
-      if (p.grad) pair_row_grad<T>(p, r, s, e, p.tk.packed ? e : p.tk.len, second ? q.gr : q.gc, lane, half);
+    o[0] = __shfl_xor(v[0], half, 64);
+    o[1] = __shfl_xor(v[1], half, 64);
+  } else {                                            // the workgroup takes one pair, half of its waves a row
+    constexpr int HW = 2;
+    v[0] = wave_sum64(v[0]);
+    v[1] = wave_sum64(v[1]);
+    if ((threadIdx.x & 63) == 0) {
+      lds[(threadIdx.x >> 6) * 2] = v[0];
+      lds[(threadIdx.x >> 6) * 2 + 1] = v[1];
+    }
+    __syncthreads();
+    const int mine = second ? 2 * HW : 0, other = 2 * HW - mine;
+    v[0] = v[1] = o[0] = o[1] = 0.0;
+#pragma unroll
+    for (int w = 0; w < HW; ++w) {
+      v[0] += lds[mine + 2 * w];
+      v[1] += lds[mine + 2 * w + 1];
+      o[0] += lds[other + 2 * w];
+      o[1] += lds[other + 2 * w + 1];
     }
   }
+  if (on) {
+    float rc, rr;
+    const PairOut q = pair_math(p, k, second ? o[0] : v[0], second ? o[1] : v[1], second ? v[0] : o[0], second ? v[1] : o[1], &rc, &rr);
+    if (lane == 0 && !second) {
+      p.rew_c[k] = rc;
+      p.rew_r[k] = rr;
+      acc[0] = q.loss; acc[1] = q.hit; acc[2] = q.z; acc[3] = q.on;
+    }
+    if (p.grad) pair_row_grad<T>(p, r, s, e, p.tk.packed ? e : p.tk.len, second ? q.gr : q.gc, lane, half);
+  }
   pair_gaps<T>(p);
-  block_sum<4, 256>(acc, lds);
+  if (per > 1) block_sum<4, 256>(acc, lds);
   if (threadIdx.x == 0) {
     if (gridDim.x == 1) pair_stats(p, acc);
     else
@@ -277,21 +277,29 @@ __global__ __launch_bounds__(256) void pairs_grad_kernel(PairP p) {
   pair_row_grad<T>(p, r, a, ve, b, r < p.pairs ? o.gc : o.gr, threadIdx.x, 256);
   pair_gaps<T>(p);
 }
-__global__ __launch_bounds__(256) void pairs_finish_kernel(PairP p) {
-  __shared__ double lds[20];
+__global__ __launch_bounds__(1024) void pairs_finish_kernel(PairP p) {
+  __shared__ double lds[17 * 4];
   double v[4] = {0, 0, 0, 0};
-  for (int b = threadIdx.x; b < p.nparts; b += 256)
+#pragma unroll 4
+  for (int b = threadIdx.x; b < p.nparts; b += 1024)
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] += p.part[(long long)b * 4 + q];
-  block_sum<4, 256>(v, lds);
+  block_sum<4, 1024>(v, lds);
   if (threadIdx.x == 0) pair_stats(p, v);
 }
 
-hipError_t launch_pairs_whole(const PairP& p, int dtype, int blocks, hipStream_t st) {
-  const dim3 g(blocks), b(256);
-  if (dtype == 0) hipLaunchKernelGGL(pairs_whole_kernel<float>, g, b, 0, st, p);
-  else if (dtype == 1) hipLaunchKernelGGL(pairs_whole_kernel<bf16_t>, g, b, 0, st, p);
-  else hipLaunchKernelGGL(pairs_whole_kernel<f16_t>, g, b, 0, st, p);
+hipError_t launch_pairs_whole(const PairP& p, int dtype, hipStream_t st) {
+  const dim3 g(p.nparts), b(256);
+#define GO(T)                                                                                          \
+  do {                                                                                                 \
+    if (p.group == 16) hipLaunchKernelGGL((pairs_whole_kernel<T, 16>), g, b, 0, st, p);                \
+    else if (p.group == 64) hipLaunchKernelGGL((pairs_whole_kernel<T, 64>), g, b, 0, st, p);           \
+    else hipLaunchKernelGGL((pairs_whole_kernel<T, 256>), g, b, 0, st, p);                             \
+  } while (0)
+  if (dtype == 0) GO(float);
+  else if (dtype == 1) GO(bf16_t);
+  else GO(f16_t);
+#undef GO
   return hipGetLastError();
 }
 template <typename T>
@@ -307,7 +315,7 @@ hipError_t launch_pairs_split(const PairP& p, int dtype, hipStream_t st) {
                                                                       : launch_pairs_split_t<f16_t>(p, st);
 }
 hipError_t launch_pairs_finish(const PairP& p, hipStream_t st) {
-  hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(1024), 0, st, p);
   return hipGetLastError();
 }
 

@@ -99,7 +99,7 @@ __device__ __forceinline__ double policy_weight(const PolicyP& p, double tokens,
   const double n = p.mode == 0 ? tokens : rows;
   return n > 0.0 ? 1.0 / n : 0.0;
 }
-// ... from the partial counts, by every wave for itself, or (one workgroup, no mask) from the rows themselves
+// ... from the partial counts, by every wave for itself, or (few rows, no mask) from the rows themselves
 __device__ __forceinline__ double policy_weight_parts(const PolicyP& p, double* lds) {
   if (p.fixed > 0.0) return p.fixed;
   if (p.tk.packed && p.mode == 0 && !p.tk.mask) {     // the offsets say how many tokens there are
@@ -123,6 +123,7 @@ __device__ __forceinline__ double policy_weight_parts(const PolicyP& p, double* 
     }
     return policy_weight(p, wave_sum64(v[0]), wave_sum64(v[1]));
   }
+#pragma unroll 8
   for (long long r = threadIdx.x; r < p.tk.rows; r += 256) {
     long long s, e;
     row_bounds(p.tk, r, &s, &e);

@@ -16,7 +16,8 @@ namespace trebi {
 // taken in float64; the sum too.
 // ---------------------------------------------------------------------------------------------------------------
 // A wave (or a workgroup, where candidates are large or few) takes a candidate, so its timestep and table rows come
-// through the scalar cache while its first elements are already on their way.
+// through the scalar cache while its first elements are already on their way.  Bound by memory from some thousand candidates
+// on: 32768 of 32 x 23 backwards, 386 MB, 71 us (5.4 TB/s: a part is read from the caches); below by the launch: 64 candidates, 3.7 us.
 template <bool BWD, int G>
 __global__ __launch_bounds__(256) void transition_kernel(TransP p) {
   __shared__ double lds[5];
@@ -98,9 +99,11 @@ __global__ __launch_bounds__(256) void transition_kernel(TransP p) {
   }
 }
 hipError_t launch_transition(const TransP& p, int backward, hipStream_t st) {
-  // a workgroup a candidate where a wave would go over its elements more than 16 times, or where there are so few
-  // candidates that one turn of every lane is what a call takes
-  const bool wide = (long long)p.H * p.D > 4096 || p.B <= 1024;
+  // A workgroup a candidate where a wave would go over its elements more than 16 times, or where there are so few
+  // candidates that what one wave goes through is what the call takes.  32 x 23 elements, forwards: 64 candidates 3.7 us, a wave
+  // each 5.1; 1024: 4.6 and 5.6; 2048: 8.1 and 7.0.  400 x 23: 64 candidates 10 and 34 us, 16384 289 and 297.  8 x 5: 1024 4.2 and 3.7.
+  const long long n = (long long)p.H * p.D;
+  const bool wide = n > 4096 || (p.B <= 1024 && n > 256);
   const long long per = wide ? 1 : 4, need = (p.B + per - 1) / per;
   const dim3 g((unsigned)(need < 8192 ? need : 8192)), b(256);
   if (backward) {

@@ -97,6 +97,11 @@ def test_preference_loss_refuses_odd_rows_and_small_workspaces():
     refused(lib.trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), PTR, need - 1, None), -4, 'workspace')
     refused(lib.trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), None, need, None), -1, 'workspace')
     assert lib.trebi_preference_loss_workspace_bytes(C.byref(tokens())) == 0
+    for rows, length in ((1 << 30, 1), (1 << 26, 5000)):                 # more workgroups than a launch has
+        d = tokens(rows=rows, len=length)
+        need = lib.trebi_preference_loss_workspace_bytes(C.byref(d))
+        assert need >= rows // 2 // 16 * 32
+        refused(lib.trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), PTR, need, None), -3, 'pairs')
 
 
 def transition(**kw):

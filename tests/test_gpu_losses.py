@@ -1,9 +1,9 @@
 """GPU: the policy loss, the preference loss and the transition log-probability against their definitions in float64
 (tests/_finetune.py), at the sizes, masks, strides and types where such kernels go wrong.
 
-Tolerances.  A gradient element is a product of fewer than 8 float32 factors, one of them an exponential (at most 2 units in the
-last place) of an argument rounded to float32 (relative 2^-24, so the exponential moves by |argument| 2^-24): with |argument| <= 16
-that is at most (2 * 2 + 8 + 16) * 2^-24 of the sum of the terms' magnitudes; 32 * 2^-24 is allowed, plus one rounding to the
+Tolerances.  A gradient element is a product of fewer than 8 float32 factors, one of them an exponential (within (|x| + 2) 2^-24 of
+its value) of an argument x rounded to float32 (relative 2^-24, so the exponential moves by |x| 2^-24): with |x| <= 8 that is at
+most (8 + 10 + 8) * 2^-24 of the sum of the terms' magnitudes; 32 * 2^-24 is allowed, plus one rounding to the
 output's type (HALF of the value, and TINY, its smallest step).  Scalars are float64 sums of such terms, rounded to float32:
 32 * 2^-24 of the sum of the terms' magnitudes."""
 import math
@@ -324,6 +324,14 @@ def test_policy_gradient_against_differences():
             assert abs((f(up) - f(dn)) / step - float(grad[i, j])) <= bound, (i, j)
 
 
+@pytest.mark.parametrize('reduction', ['token', 'sequence'])
+@pytest.mark.parametrize('layout', ['lengths', 'packed', 'packed-mask', 'mask'])
+def test_policy_loss_counts_rows_on_both_sides_of_every_choice(layout, reduction):
+    """Few rows are counted where they are needed, many by a kernel of their own; the same for calls of one workgroup."""
+    for rows, length in ((2047, 5), (2048, 5), (2049, 5), (5000, 3), (4096, 1), (4097, 1), (300, 31)):
+        run_policy(layout, rows, length, 'float32', seed=rows, reduction=reduction, kl_coef=0.05)
+
+
 # ------------------------------------------------------------------------------------------------- preference loss
 def run_pairs(layout, P, length, dtype, seed=0, strided=False, has_ref=True, weights=False, **kw):
     from trebi_amd.losses import preference_loss
@@ -388,6 +396,20 @@ def test_preference_loss_with_rows_split_over_workgroups(layout):
 def test_preference_loss_many_pairs_and_every_group_size():
     for P, length in ((5000, 3), (600, 200), (513, 1500), (520, 4200)):
         run_pairs('all', P, length, 'bfloat16', seed=P, average=True)
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+def test_preference_loss_on_both_sides_of_every_choice(layout):
+    """Threads of a pair by the rows' lengths and the pairs' number; rows split over workgroups from 8192 tokens on."""
+    for n, (P, length) in enumerate([(5, 127), (5, 129), (1023, 130), (1025, 130), (4097, 130), (4095, 130), (1025, 513), (2, 8192), (2, 8193),
+                                     (70, 8200), (60, 8200)]):
+        run_pairs(layout, P, length, 'float16' if n % 2 else 'float32', seed=n, average=True, weights=bool(n % 3))
+
+
+@pytest.mark.parametrize('strided', ['transposed', 'slice', 'shifted'])
+def test_preference_loss_reads_views_of_split_rows(strided):
+    for layout in ('all', 'lengths', 'mask'):
+        run_pairs(layout, 2, 9000, 'bfloat16', strided=strided, average=True)
 
 
 @pytest.mark.parametrize('strided', ['transposed', 'slice', 'shifted'])
