@@ -446,6 +446,7 @@ static int trainer_repack(trebi_trainer* tr, hipStream_t st) {
 extern "C" int trebi_trainer_repack(trebi_trainer* tr, void* stream) {
   if (!tr || !tr->bound) return fail(TREBI_BAD_ARG, "trainer is null or not bound");
   HIPCHK(hipSetDevice(tr->ctx->device));
+  tr->fwd_x = nullptr;                             // a backward would run on other parameters than its forward
   return trainer_repack(tr, (hipStream_t)stream);
 }
 
@@ -539,6 +540,7 @@ extern "C" int trebi_trainer_bind(trebi_trainer* tr, float* params, float* grads
 
 extern "C" int trebi_trainer_set_precision(trebi_trainer* tr, int mode, int min_batch) {
   if (!tr) return fail(TREBI_BAD_ARG, "null trainer");
+  tr->fwd_x = nullptr;
   if (int e = trebi_net_set_precision(tr->net, mode, min_batch)) return e;
   if (tr->bound && mode == 1)
     if (int e = net_refresh_bf16(tr->net, 0)) return e;

@@ -214,6 +214,18 @@ def test_halves_refuse_misuse():
         eng.log_prob(x, x[:3], t)
 
 
+def test_backward_refused_after_the_parameters_or_the_precision_changed():
+    diff, _ = model()
+    eng = diff.train_engine(4)
+    x, t = torch.zeros(4, H, D, device='cuda'), torch.ones(4, dtype=torch.long, device='cuda')
+    for change in (eng.repack, lambda: eng.set_precision('bf16x3', 0), lambda: eng.set_precision('f32'),
+                   lambda: eng.step(1, 1e-3), lambda: eng.step(2, 1e-3, max_grad_norm=1.0)):
+        eng.forward(x, t)
+        change()
+        with pytest.raises(RuntimeError, match='trebi_trainer_forward'):
+            eng.backward(x)
+
+
 def test_clipped_step_equals_a_step_on_the_scaled_gradient():
     a, sd = model()
     b, _ = model()
