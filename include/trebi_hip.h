@@ -356,8 +356,9 @@ int trebi_trainer_backward(trebi_trainer* tr, const float* x, const int64_t* t, 
 /* ---- fine-tuning ------------------------------------------------------------------
  * What follows the imitation of the training step above: policy-gradient and preference fine-tuning of the denoiser,
  * and the clipping that keeps such steps stable.  No counterpart in the reference.  These calls allocate nothing, keep
- * no state and only enqueue (graph-capturable); tables and workspaces are the caller's, one per call in flight.  Sums
- * are taken in float64 and in a fixed order: results do not change from run to run. */
+ * no state and only enqueue (graph-capturable); tables and workspaces are the caller's, one per call in flight (256-byte
+ * aligned; where a *_workspace_bytes call returns 0, workspace may be null).  Sums are taken in float64 and in a fixed
+ * order: results do not change from run to run. */
 typedef enum { TREBI_F32 = 0, TREBI_BF16 = 1, TREBI_F16 = 2 } trebi_dtype;
 
 /* Global gradient norm over many tensors (each contiguous, aligned to its type; numels may be 0), and clipping:
