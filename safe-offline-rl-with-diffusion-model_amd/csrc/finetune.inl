@@ -50,7 +50,7 @@ int grad_totals(int n, const int64_t* numels, long long* total, long long* chunk
 
 // From this many bytes on the 256 MB cache cannot hand a set from one kernel to the next: such sets are read (for the norm
 // alone) and written past the caches.  Norm of 366 MB 59 us, through them 67; 976 MB 151 and 172; 244 MB: 42 both ways.
-// Clipping 800 MB of bfloat16 in place: 315 us, through them 353.
+// Clipping 200 M bfloat16 into float32: 315 us, through them 353.
 constexpr long long GRAD_STREAM = 256ll << 20;
 
 int grad_args(trebi_ctx* ctx, const trebi_grad_set* set, const void* table, int norm_type, float grad_scale, void* ws,

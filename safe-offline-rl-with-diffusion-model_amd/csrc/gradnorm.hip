@@ -4,10 +4,10 @@
 //   out = c * g                           s: the factor that takes a loss scale off (1 / loss scale)
 //
 // Bound by memory: every gradient is read once for the norm and once more (partly still in the 256 MB cache) for the
-// scaled copy.  Norm of 1.07 GB of float32: 160 us, 6.7 TB/s.  400 M bfloat16 clipped in place: 69 us for the norm (the 800 MB are
-// partly in the cache: 11.6 TB/s) and 247 us to read and write them (6.5 TB/s).  4.25 M float32 into a flat copy: 5.7 and 7.2 us, of which
-// the memory takes 6.6 (a copy's rate): what is left are the launches and the partial sums.  The tensors are cut into chunks on the host and the workgroups walk chunks, so that 400 tensors cost the same
-// two launches as one.  The sum is held in float64: no length and no magnitude (1e-30 .. 1e30) loses digits or overflows.
+// scaled copy.  Norm of 1.07 GB of float32: 160 us, 6.7 TB/s.  200 M bfloat16 scaled into float32: 69 us for the norm (400 MB, 5.8
+// TB/s) and 247 us for the copy (1.2 GB, 4.9 TB/s, a large copy's rate).  3.96 M float32 into a flat copy: 5.7 and 7.2 us, of which the
+// memory takes 6.6: what is left are the launches and the partial sums.  The tensors are cut into chunks on the host and the
+// workgroups walk chunks, so that 400 tensors cost the same two launches as one.  The sum is held in float64: no length and no magnitude (1e-30 .. 1e30) loses digits or overflows.
 // Each workgroup leaves one partial sum; the kernel that scales adds the partials up itself, every workgroup in the same
 // order, so no atomics, no order that changes from run to run, and no third launch.
 #include "finetune.h"
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(GradP p) {
 }
 
 // The same for sets of one chunk a workgroup (up to 8 M elements), which latency bounds: the chunk's loads are on their way
-// while the partial sums are added up.  4.25 M float32 into a flat copy 7.2 us, with the kernel above 8.6.
+// while the partial sums are added up.  3.96 M float32 into a flat copy 7.2 us, with the kernel above 8.6.
 __global__ __launch_bounds__(256) void grad_scale_small_kernel(GradP p) {
   __shared__ double lds[4];
   typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(2)));
