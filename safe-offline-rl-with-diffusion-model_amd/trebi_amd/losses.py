@@ -51,9 +51,9 @@ def _like(name, v, logp):
     """Another per-token tensor of logp's shape, type and device."""
     if v.shape != logp.shape:
         raise ValueError(f'{name} has shape {tuple(v.shape)}, logp {tuple(logp.shape)}')
-    if v.dtype != logp.dtype:
+    if v.dtype is not logp.dtype:
         raise TypeError(f'{name} has type {v.dtype}, logp {logp.dtype}')
-    if v.device != logp.device:
+    if v.get_device() != logp.get_device():
         raise RuntimeError(f'{name} is on {v.device}, logp on {logp.device}')
     return v
 
@@ -131,7 +131,7 @@ def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, le
     if logp_ref is not None:
         _like('logp_ref', logp_ref, logp)
     d, rows, keep = _token_desc(logp, mask, lengths, cu_seqlens)
-    if advantages.dtype != torch.float32 or advantages.device != dev:
+    if advantages.dtype is not torch.float32 or advantages.get_device() != logp.get_device():
         raise TypeError(f'advantages must be float32 on {dev}, got {advantages.dtype} on {advantages.device}')
     packed = cu_seqlens is not None
     if packed:
@@ -153,7 +153,7 @@ def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, le
             adv_stride = advantages.stride()                        # (column stride 0: one a row, expanded)
         else:
             raise ValueError(f'advantages must be [{rows}] or {tuple(logp.shape)}, got {tuple(advantages.shape)}')
-    grad = torch.empty(logp.shape, dtype=logp.dtype, device=dev) if want_grad else None
+    grad = torch.empty_like(logp, memory_format=torch.contiguous_format) if want_grad else None
     if rows == 0 or logp.numel() == 0:
         z = torch.zeros(5, device=dev).unbind()
         return PolicyLoss(z[0], None if grad is None else grad.zero_().reshape(shape), *z[1:])
@@ -217,7 +217,7 @@ def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=
         strides = [(0, 1)] * 2
     else:
         strides = [logp.stride(), (0, 1) if logp_ref is None else logp_ref.stride()]
-    grad = torch.empty(logp.shape, dtype=logp.dtype, device=dev) if want_grad else None
+    grad = torch.empty_like(logp, memory_format=torch.contiguous_format) if want_grad else None
     if P == 0:
         z = torch.zeros(3, device=dev).unbind()
         e = torch.empty(0, device=dev)
@@ -242,8 +242,8 @@ def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=
 # ------------------------------------------------------------------------------------------- denoise transitions
 def _rows(name, v, shape, device):
     """float32 [B, H, D] whose candidates are contiguous (a slice of a chain keeps its stride), copied otherwise."""
-    if v.shape != shape or v.device != device:
-        raise ValueError(f'{name} is {tuple(v.shape)} on {v.device}, expected {tuple(shape)} on {device}')
+    if v.shape != shape or v.get_device() != device:
+        raise ValueError(f'{name} is {tuple(v.shape)} on {v.device}, expected {tuple(shape)} on cuda:{device}')
     if v.dtype is not torch.float32:
         raise TypeError(f'{name} must be float32, got {v.dtype}')
     s = v.stride()
@@ -253,13 +253,9 @@ def _rows(name, v, shape, device):
     return v, s[0]
 
 
-_TABLES = ('posterior_log_variance_clipped', 'posterior_mean_coef1', 'posterior_mean_coef2')
-_NOISE_TABLES = ('sqrt_recip_alphas_cumprod', 'sqrt_recipm1_alphas_cumprod')
-
-
 def _transition(model, pred, x, x_prev, t, cond_keys):
-    dev, shape, T = pred.device, pred.shape, model.n_timesteps
-    if dev.type != 'cuda':
+    shape, dev, T, f32 = pred.shape, pred.get_device(), model.n_timesteps, torch.float32
+    if not pred.is_cuda:
         raise RuntimeError('trebi_amd computes transition log-probabilities on an MI355X only; there is no CPU path')
     if len(shape) != 3 or shape[2] != model.transition_dim:
         raise ValueError(f'pred must be [batch, horizon, {model.transition_dim}], got {tuple(shape)}')
@@ -271,23 +267,28 @@ def _transition(model, pred, x, x_prev, t, cond_keys):
         t = torch.as_tensor(t)
     if t.dim() == 0:
         t = t.expand(B)
-    if t.shape != (B,) or t.is_floating_point():
+    if t.dim() != 1 or t.numel() != B or t.is_floating_point():
         raise ValueError(f't must be [{B}] integers, got {t.dtype} {tuple(t.shape)}')
     if not t.is_cuda and B and not (0 <= int(t.min()) and int(t.max()) < T):
         raise RuntimeError(f'timesteps must lie in [0, {T})')
-    if t.dtype is not torch.int64 or t.device != dev:
-        t = t.to(dev, torch.int64)
+    if t.dtype is not torch.int64 or t.get_device() != dev:
+        t = t.to(pred.device, torch.int64)
     t = t.contiguous()
-    keys = sorted(int(k) for k in cond_keys)
-    if len(keys) > 4:
-        raise RuntimeError('at most 4 conditioned timesteps are supported')
-    ptrs = []
-    for n in _TABLES + _NOISE_TABLES if model.predict_epsilon else _TABLES:
-        tab = getattr(model, n)
-        if tab.device != dev or tab.dtype is not torch.float32 or tab.shape != (T,) or not tab.is_contiguous():
-            raise RuntimeError(f'{n} must be a contiguous float32 [{T}] on {dev}')
-        ptrs.append(tab.data_ptr())
-    ptrs += [0] * (5 - len(ptrs))
+    keys = tuple(cond_keys)
+    if keys != (0,):
+        keys = tuple(sorted(int(k) for k in keys))
+        if len(keys) > 4:
+            raise RuntimeError('at most 4 conditioned timesteps are supported')
+    tables = [model.posterior_log_variance_clipped, model.posterior_mean_coef1, model.posterior_mean_coef2]
+    if model.predict_epsilon:
+        tables += [model.sqrt_recip_alphas_cumprod, model.sqrt_recipm1_alphas_cumprod]
+    for tab in tables:
+        if tab.get_device() != dev or tab.dtype is not f32 or tab.dim() != 1 or tab.numel() != T or not tab.is_contiguous():
+            raise RuntimeError(f"the model's schedule must be contiguous float32 [{T}] tensors on cuda:{dev}, one is {tab.dtype} "
+                               f'{tuple(tab.shape)} on {tab.device}')
+    ptrs = [tab.data_ptr() for tab in tables]
+    if len(ptrs) == 3:
+        ptrs += [0, 0]
     d = _TRANSITION.pack(H, D, model.action_dim, model.observation_dim, T, 1 if model.clip_denoised else 0, len(keys),
                          *keys, *[0] * (4 - len(keys)), ps, xs, qs, *ptrs)
     return d, pred, x, x_prev, t
@@ -314,10 +315,10 @@ def transition_log_prob_grad(model, pred, x, x_prev, t, grad, cond_keys=(0,)):
     """grad[b] * d transition_log_prob[b] / d pred, [B, H, D]; `grad`: float32 [B], d loss / d log-probability."""
     d, pred, x, x_prev, t = _transition(model, pred, x, x_prev, t, cond_keys)
     B, dev = pred.shape[0], pred.device
-    if grad.shape != (B,) or grad.dtype is not torch.float32 or grad.device != dev:
+    if grad.dim() != 1 or grad.numel() != B or grad.dtype is not torch.float32 or grad.get_device() != pred.get_device():
         raise ValueError(f'grad must be float32 [{B}] on {dev}, got {grad.dtype} {tuple(grad.shape)} on {grad.device}')
     grad = grad.contiguous()
-    out = torch.empty(pred.shape, device=dev)
+    out = torch.empty_like(pred, memory_format=torch.contiguous_format)
     if B:
         rc = _lib.lib().trebi_transition_logp_grad(_lib.ctx(dev.index or 0), d, pred.data_ptr(), x.data_ptr(), x_prev.data_ptr(),
                                                    t.data_ptr(), grad.data_ptr(), B, out.data_ptr(), _lib.stream(dev))
