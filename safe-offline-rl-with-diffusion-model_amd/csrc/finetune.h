@@ -64,7 +64,7 @@ struct PolicyP {
   int early;                               // load tokens before it is known which of them count
   int flat;                                // every view is contiguous and rows are not tiny: vector loads across rows
 };
-hipError_t launch_token_counts(const PolicyP& p, hipStream_t st);
+hipError_t launch_token_counts(PolicyP& p, hipStream_t st);     // sets p.nnp
 hipError_t launch_policy(const PolicyP& p, int dtype, int blocks, hipStream_t st);
 hipError_t launch_policy_finish(const PolicyP& p, int blocks, hipStream_t st);
 

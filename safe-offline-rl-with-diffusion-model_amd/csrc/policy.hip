@@ -27,7 +27,16 @@ __global__ __launch_bounds__(256) void token_count_kernel(TokenP t, int G, NormP
       else if (t.mcs == 1) {
         const unsigned char* m = t.mask + (t.packed ? 0 : r * t.mrs);
         typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(1)));
-        for (long long i = s + gl * 16; i < e; i += G * 16) {
+        const long long step = (long long)G * 16;
+        long long i = s + gl * 16;
+        for (; i + 3 * step + 16 <= e; i += 4 * step) {           // (few long rows: four loads on their way)
+          u4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = *(const TREBI_GLOBAL u4*)(m + i + u * step);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) c += bytes_set(v[u].x) + bytes_set(v[u].y) + bytes_set(v[u].z) + bytes_set(v[u].w);
+        }
+        for (; i < e; i += step) {
           if (i + 16 <= e) {
             const u4 v = *(const TREBI_GLOBAL u4*)(m + i);
             c += bytes_set(v.x) + bytes_set(v.y) + bytes_set(v.z) + bytes_set(v.w);
@@ -62,28 +71,38 @@ static int group_of(const TokenP& t) {
   const long long len = t.packed ? (t.n + t.rows - 1) / t.rows : t.len;
   return !t.mask ? 1 : len <= 64 ? 4 : len <= 256 ? 16 : len <= 1024 ? 64 : 256;
 }
-// Where only the tokens of a whole contiguous mask are wanted, rows do not matter
-__global__ __launch_bounds__(256) void mask_count_kernel(const unsigned char* m, long long n, NormPart* np) {
+// Where only the tokens of a contiguous mask are wanted, between the first and the last offset, rows do not matter
+__global__ __launch_bounds__(256) void mask_count_kernel(TokenP t, NormPart* np) {
   __shared__ double lds[5];
   typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(1)));
+  long long s = 0, e = t.n;
+  if (t.packed) {
+    s = uniform_load(t.cu);
+    e = uniform_load(t.cu + t.rows);
+    s = s < 0 ? 0 : s;
+    e = e > t.n ? t.n : e;
+  }
+  const unsigned char* m = t.mask;
   const long long step = (long long)gridDim.x * 4096;
   long long c = 0;
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 16; i < n; i += step) {
-    if (i + 16 <= n) {
+  for (long long i = s + ((long long)blockIdx.x * 256 + threadIdx.x) * 16; i < e; i += step) {
+    if (i + 16 <= e) {
       const u4 v = *(const TREBI_GLOBAL u4*)(m + i);
       c += bytes_set(v.x) + bytes_set(v.y) + bytes_set(v.z) + bytes_set(v.w);
     } else {
-      for (long long j = i; j < n; ++j) c += m[j] != 0;
+      for (long long j = i; j < e; ++j) c += m[j] != 0;
     }
   }
   double v[1] = {(double)c};
   block_sum<1, 256>(v, lds);
   if (threadIdx.x == 0) np[blockIdx.x] = {(long long)v[0], 0};
 }
-hipError_t launch_token_counts(const PolicyP& p, hipStream_t st) {
+hipError_t launch_token_counts(PolicyP& p, hipStream_t st) {
   const TokenP& t = p.tk;
-  if (t.mask && !t.packed && !t.lengths && p.mode == 0 && t.mcs == 1 && t.mrs == t.len)
-    hipLaunchKernelGGL(mask_count_kernel, dim3(p.nnp), dim3(256), 0, st, t.mask, t.n, p.np);
+  const bool whole = t.mask && !t.lengths && p.mode == 0 && (t.packed || (t.mcs == 1 && t.mrs == t.len));
+  const long long want = whole ? (t.n + 4095) / 4096 : t.mask ? t.rows : (t.rows + 255) / 256;
+  p.nnp = (int)(want < COUNT_BLOCKS ? want : COUNT_BLOCKS);
+  if (whole) hipLaunchKernelGGL(mask_count_kernel, dim3(p.nnp), dim3(256), 0, st, t, p.np);
   else
     hipLaunchKernelGGL(token_count_kernel, dim3(p.nnp), dim3(256), 0, st, t, group_of(t), p.np, p.counts);
   return hipGetLastError();

@@ -324,6 +324,41 @@ def test_policy_gradient_against_differences():
             assert abs((f(up) - f(dn)) / step - float(grad[i, j])) <= bound, (i, j)
 
 
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+@pytest.mark.parametrize('strided', [False, 'columns', 'mask'])
+def test_policy_loss_rows_of_one_token(strided, dtype):
+    """[N, 1] and [N], with a mask, a stride between the rows, advantages one a row or one for all: as the definition says, for both means."""
+    from trebi_amd.losses import policy_loss
+    for N in (1, 7, 8, 9, 4096, 4097, 70001):
+        g = torch.Generator().manual_seed(N)
+        logp = -torch.rand(N, 3, generator=g) * 3
+        old, ref = logp + 0.3 * torch.randn(N, 3, generator=g), logp + 0.3 * torch.randn(N, 3, generator=g)
+        adv, mask = torch.randn(N, generator=g), torch.rand(N, 3, generator=g) < 0.7
+        pick = (lambda v: v[:, 1:2]) if strided == 'columns' else (lambda v: v[:, 1:2].contiguous())
+        lp, o, r = (pick(v.to(DT[dtype]).cuda()) for v in (logp, old, ref))
+        m = mask.cuda()[:, 1:2] if strided else mask.cuda()[:, 1:2].contiguous()
+        for use in (None, m):
+            on = np.ones(N, bool) if use is None else mask[:, 1].numpy()
+            out = [policy_loss(lp, adv.cuda(), o, r, mask=use, kl_coef=0.05, reduction=red) for red in ('token', 'sequence')]
+            flat = policy_loss(lp[:, 0].contiguous()[None], adv.cuda()[None], o[:, 0].contiguous()[None], r[:, 0].contiguous()[None],
+                               mask=None if use is None else use[:, 0].contiguous()[None], kl_coef=0.05)
+            one = policy_loss(lp[:, 0], adv.cuda(), o[:, 0], r[:, 0], mask=None if use is None else use[:, 0], kl_coef=0.05)
+            for v in out + [one]:
+                assert v.grad.shape == (lp.shape if v is not one else (N,))
+                assert torch.allclose(v.grad.reshape(-1).double(), flat.grad[0].double(), rtol=2 * F.HALF[dtype] + ULP, atol=ULP / max(on.sum(), 1))
+                assert abs(float(v.loss) - float(flat.loss)) <= 2 * ULP * (1 + abs(float(flat.loss)))
+    a = policy_loss(lp, torch.ones(1, device='cuda').expand(N), o, r)          # one advantage for all: stride 0
+    b = policy_loss(lp, torch.ones(N, device='cuda'), o, r)
+    assert torch.allclose(a.grad.float(), b.grad.float(), rtol=2 * F.HALF[dtype] + ULP, atol=0)
+
+
+@pytest.mark.parametrize('reduction', ['token', 'sequence'])
+@pytest.mark.parametrize('layout', ['mask', 'packed-mask'])
+def test_policy_loss_counts_long_masked_rows(layout, reduction):
+    run_policy(layout, 2, 70003, 'float32', seed=5, reduction=reduction, kl_coef=0.05)
+    run_policy(layout, 1, 20011, 'bfloat16', seed=6, reduction=reduction)
+
+
 @pytest.mark.parametrize('dtype', list(DT))
 @pytest.mark.parametrize('which', ['all', 'lengths', 'mask'])
 def test_policy_loss_sums_of_equal_ratios_have_no_bias(which, dtype):
