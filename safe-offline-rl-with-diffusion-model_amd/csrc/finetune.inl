@@ -78,7 +78,8 @@ int token_args(const trebi_token_desc& d, TokenP* t) {
     if (!d.cu_seqlens) return fail(TREBI_BAD_ARG, "packed tokens need cu_seqlens");
     if (d.rows < 1) return fail(TREBI_BAD_SHAPE, "packed tokens need at least one sequence");
     if (d.lengths) return fail(TREBI_BAD_ARG, "lengths belong to padded rows");
-    if (d.len > 0x7fffffff) return fail(TREBI_UNSUPPORTED_CONFIG, "cu_seqlens is 32-bit: at most 2^31 - 1 packed tokens");
+    if (d.len > 0x7fffffff || d.rows > 0x7fffff00)
+      return fail(TREBI_UNSUPPORTED_CONFIG, "cu_seqlens is 32-bit: at most 2^31 - 1 packed tokens, fewer sequences");
     if (d.mask && d.mask_col_stride != 1) return fail(TREBI_BAD_ARG, "a packed mask is contiguous");
   } else {
     if (d.cu_seqlens) return fail(TREBI_BAD_ARG, "cu_seqlens belongs to packed tokens");

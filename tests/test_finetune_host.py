@@ -59,6 +59,14 @@ def test_token_descriptions_refused(change, code, word):
     refused(_lib.lib().trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), PTR, 1 << 40, None), code, word)
 
 
+def test_more_packed_sequences_than_32_bits_count_are_refused():
+    lib = _lib.lib()
+    for rows, code in ((0x7fffffff, -3), (1 << 39, -3)):
+        d = tokens(packed=1, cu_seqlens=PTR, rows=rows)
+        refused(lib.trebi_policy_loss(CTX, C.byref(d), C.byref(policy()), PTR, 1 << 50, None), code, 'fewer sequences')
+        refused(lib.trebi_preference_loss(CTX, C.byref(d), C.byref(pairs()), PTR, 1 << 50, None), code, 'fewer sequences')
+
+
 def test_policy_loss_refuses_masked_rows_beyond_32_bits():
     d, q = tokens(rows=1, len=1 << 31, mask=PTR), policy(reduction=1)
     refused(_lib.lib().trebi_policy_loss(CTX, C.byref(d), C.byref(q), PTR, 1 << 40, None), -3, 'masked')
