@@ -52,7 +52,7 @@ class GradClipper:
         dtypes = (C.c_int * n)(*[_DTYPES[t.dtype] for t in self.tensors])
         lib = _lib.lib()
         nbytes = lib.trebi_grad_set_bytes(n, numels)
-        host = torch.empty(max(nbytes, 1), dtype=torch.uint8)
+        host = torch.empty(max(nbytes, 1), dtype=torch.uint8, device='cpu')
         self.set = _lib.GradSet()
         _lib.check(lib.trebi_grad_set_fill(n, ptrs, numels, dtypes, _lib.ptr(host), nbytes, C.byref(self.set)))
         self.table = host.to(self.device)
@@ -64,7 +64,7 @@ class GradClipper:
     def _buffers(self):
         """A workspace of this call's own (two calls may run at once), the norm, the stream."""
         ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
-        return ws, torch.empty((), device=self.device), _lib.stream(self.device)
+        return ws, torch.empty((), dtype=torch.float32, device=self.device), _lib.stream(self.device)
 
     def norm(self, grad_scale=1.0):
         """grad_scale * the norm, a device scalar."""
@@ -82,7 +82,7 @@ class GradClipper:
     def clip_into(self, max_norm, grad_scale=1.0, out=None):
         """(flat, norm): the scaled gradients as one float32 tensor in the tensors' order; the gradients keep their values."""
         if out is None:
-            out = torch.empty(self.total, device=self.device)
+            out = torch.empty(self.total, dtype=torch.float32, device=self.device)
         elif out.shape != (self.total,) or out.dtype != torch.float32 or out.device != self.device or not out.is_contiguous():
             raise RuntimeError(f'out must be a contiguous float32 [{self.total}] on {self.device}')
         else:
@@ -103,7 +103,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
-        return torch.tensor(0.0)
+        return torch.tensor(0.0, dtype=torch.float32, device='cpu')
     clipper = GradClipper(grads, norm_type)
     if error_if_nonfinite:
         norm = clipper.norm()

@@ -155,9 +155,9 @@ def policy_loss(logp, advantages, logp_old=None, logp_ref=None, *, mask=None, le
             raise ValueError(f'advantages must be [{rows}] or {tuple(logp.shape)}, got {tuple(advantages.shape)}')
     grad = torch.empty_like(logp, memory_format=torch.contiguous_format) if want_grad else None
     if rows == 0 or logp.numel() == 0:
-        z = torch.zeros(5, device=dev).unbind()
+        z = torch.zeros(5, dtype=torch.float32, device=dev).unbind()
         return PolicyLoss(z[0], None if grad is None else grad.zero_().reshape(shape), *z[1:])
-    stats = torch.empty(5, device=dev)
+    stats = torch.empty(5, dtype=torch.float32, device=dev)
     lib = _lib.lib()
     ws_bytes = lib.trebi_policy_loss_workspace_bytes(d)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
@@ -219,10 +219,10 @@ def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=
         strides = [logp.stride(), (0, 1) if logp_ref is None else logp_ref.stride()]
     grad = torch.empty_like(logp, memory_format=torch.contiguous_format) if want_grad else None
     if P == 0:
-        z = torch.zeros(3, device=dev).unbind()
-        e = torch.empty(0, device=dev)
+        z = torch.zeros(3, dtype=torch.float32, device=dev).unbind()
+        e = torch.empty(0, dtype=torch.float32, device=dev)
         return PreferenceLoss(z[0], None if grad is None else grad.zero_().reshape(shape), e, e.clone(), z[1], z[2])
-    out = torch.empty(2 * P + 3, device=dev)
+    out = torch.empty(2 * P + 3, dtype=torch.float32, device=dev)
     lib = _lib.lib()
     ws_bytes = lib.trebi_preference_loss_workspace_bytes(d)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
@@ -302,7 +302,7 @@ def transition_log_prob(model, pred, x, x_prev, t, cond_keys=(0,)):
     t is not checked here: the kernels cut it to the tables.)"""
     d, pred, x, x_prev, t = _transition(model, pred, x, x_prev, t, cond_keys)
     B, dev = pred.shape[0], pred.device
-    logp = torch.empty(B, device=dev)
+    logp = torch.empty(B, dtype=torch.float32, device=dev)
     if B:
         rc = _lib.lib().trebi_transition_logp(_lib.ctx(dev.index or 0), d, pred.data_ptr(), x.data_ptr(), x_prev.data_ptr(),
                                               t.data_ptr(), B, logp.data_ptr(), _lib.stream(dev))

@@ -74,17 +74,17 @@ class TrainEngine:
             _lib.check(_lib.lib().trebi_trainer_create(_lib.ctx(dev.index or 0), C.byref(d), self.max_batch, C.byref(h)))
         self.h = h
         assert _lib.lib().trebi_trainer_param_count(h) == P
-        self.params = torch.empty(P, device=dev)
-        self.grads = torch.zeros(P, device=dev)
-        self.exp_avg = torch.zeros(P, device=dev)
-        self.exp_avg_sq = torch.zeros(P, device=dev)
+        self.params = torch.empty(P, dtype=torch.float32, device=dev)
+        self.grads = torch.zeros(P, dtype=torch.float32, device=dev)
+        self.exp_avg = torch.zeros(P, dtype=torch.float32, device=dev)
+        self.exp_avg_sq = torch.zeros(P, dtype=torch.float32, device=dev)
         _flatten_into(unet, self.names, self.params)
         self.ema = None
         if ema_model is not None:
-            self.ema = torch.empty(P, device=dev)
+            self.ema = torch.empty(P, dtype=torch.float32, device=dev)
             _flatten_into(ema_model.model, self.names, self.ema)
             self.ema_unet = ema_model.model
-        self.loss_acc = torch.zeros(2, device=dev)
+        self.loss_acc = torch.zeros(2, dtype=torch.float32, device=dev)
         tabs = [t.detach().to('cpu', torch.float32).contiguous() for t in
                 (diffusion.loss_fn.weights, diffusion.sqrt_alphas_cumprod, diffusion.sqrt_one_minus_alphas_cumprod)]
         fp = lambda t: C.cast(t.data_ptr(), _lib.c_float_p)
@@ -126,7 +126,7 @@ class TrainEngine:
         """One micro-batch: grads += grad_scale * d loss/d params.  Returns a device tensor [loss, a0_loss]."""
         B = x.shape[0]
         if B == 0:
-            return torch.zeros(2, device=self.device)
+            return torch.zeros(2, dtype=torch.float32, device=self.device)
         if sorted(int(k) for k in cond.keys()) != self.cond_keys:
             raise RuntimeError(f'conditioned timesteps {sorted(cond.keys())} differ from the engine\'s {self.cond_keys}')
         f32 = lambda v: torch.as_tensor(v, device=self.device, dtype=torch.float32).contiguous()
@@ -138,7 +138,7 @@ class TrainEngine:
                 raise RuntimeError(f'cond has shape {tuple(c.shape)}, expected {(B, self.diffusion.observation_dim)}')
         if x.shape != (B, self.diffusion.horizon, self.diffusion.transition_dim) or noise.shape != x.shape or t.shape != (B,):
             raise RuntimeError('x / noise must be [batch, horizon, transition_dim] and t [batch]')
-        out = torch.zeros(2, device=self.device)
+        out = torch.zeros(2, dtype=torch.float32, device=self.device)
         _lib.check(_lib.lib().trebi_trainer_accumulate(self.h, _lib.ptr(x), _lib.ptr_array(cts), _lib.ptr(t), _lib.ptr(noise),
                                                        B, float(grad_scale), _lib.ptr(out), self._stream()))
         return out
@@ -203,7 +203,7 @@ class TrainEngine:
         for lo, hi in parts:
             pred = self.forward(x[lo:hi], t[lo:hi])
             logp.append(transition_log_prob(m, pred, x[lo:hi], x_prev[lo:hi], t[lo:hi], self.cond_keys))
-        logp = torch.cat(logp) if logp else torch.empty(0, device=self.device)
+        logp = torch.cat(logp) if logp else torch.empty(0, dtype=torch.float32, device=self.device)
         out = loss(logp.view(lead), (t > 0).view(lead))       # the last step (t = 0) adds no noise: nothing to learn from
         g = out.grad.reshape(-1)
         for k, (lo, hi) in enumerate(reversed(parts)):
@@ -222,7 +222,7 @@ class TrainEngine:
         out = [transition_log_prob(self.diffusion, self.forward(x[lo:hi], t[lo:hi]), x[lo:hi], x_prev[lo:hi], t[lo:hi], self.cond_keys)
                for lo, hi in self._parts(len(x))]
         self._kept = None
-        return (torch.cat(out) if out else torch.empty(0, device=self.device)).view(lead)
+        return (torch.cat(out) if out else torch.empty(0, dtype=torch.float32, device=self.device)).view(lead)
 
     @torch.no_grad()
     def accumulate_policy(self, x, x_prev, t, advantages, logp_old=None, logp_ref=None, *, mask=None, grad_scale=1.0, **loss):
@@ -259,7 +259,7 @@ class TrainEngine:
         if max_grad_norm is None:
             _lib.check(_lib.lib().trebi_trainer_step(*args, self._stream()))
         else:
-            norm = torch.empty((), device=self.device)
+            norm = torch.empty((), dtype=torch.float32, device=self.device)
             _lib.check(_lib.lib().trebi_trainer_step_clipped(*args, float(max_grad_norm), _lib.ptr(norm), self._stream()))
         for net in (self.unet, getattr(self, 'ema_unet', None)):      # planning with these modules must re-pack
             if net is not None:
@@ -366,7 +366,7 @@ class Trainer:
                 t, noise = batch[2], batch[3]
             else:
                 t = torch.randint(0, self.model.n_timesteps, (B,), device=dev).long()
-                noise = torch.randn(tuple(x.shape), device=dev)
+                noise = torch.randn(tuple(x.shape), dtype=torch.float32, device=dev)
             Bg = global_batch_sizes[i] if global_batch_sizes is not None else B * world
             scale = (B / Bg if Bg else 0.0) / len(batches)                              # training.py:115
             last = overlap and i == len(batches) - 1
