@@ -194,7 +194,7 @@ def _ddpm_step(model, x, cond, t, noise):
 @torch.no_grad()
 def default_sample_fn(model, x, cond, t, guide=None, noise=None):      # diffusion.py:19-29
     out = _ddpm_step(model, x, cond, t, _noise_for(x, t, noise))
-    values = torch.zeros(len(x), device=x.device)
+    values = torch.zeros(len(x), dtype=torch.float32, device=x.device)
     return out, values, values
 
 
@@ -407,11 +407,11 @@ class GaussianDiffusion(nn.Module):
             T = self.n_timesteps
             self._samplers[key] = dict(
                 h=h,
-                noise=torch.empty(T + 1, B, H, D, device=device),
-                x=torch.empty(B, H, D, device=device),
-                values=torch.empty(B, device=device), costs=torch.empty(B, device=device),
-                thr=torch.zeros(B, device=device),
-                cond=[torch.empty(B, self.observation_dim, device=device) for _ in keys],
+                noise=torch.empty(T + 1, B, H, D, dtype=torch.float32, device=device),
+                x=torch.empty(B, H, D, dtype=torch.float32, device=device),
+                values=torch.empty(B, dtype=torch.float32, device=device), costs=torch.empty(B, dtype=torch.float32, device=device),
+                thr=torch.zeros(B, dtype=torch.float32, device=device),
+                cond=[torch.empty(B, self.observation_dim, dtype=torch.float32, device=device) for _ in keys],
                 chain=None)
         return self._samplers[key]
 
@@ -450,9 +450,9 @@ class GaussianDiffusion(nn.Module):
         device = self.betas.device
         B, H, D = shape
         if B == 0:                                  # empty batch: nothing to plan (torch would return empty tensors)
-            e = torch.empty(0, device=device)
-            chain = torch.empty(self.n_timesteps + 1, 0, H, D, device=device) if return_chain else None
-            return torch.empty(0, H, D, device=device), e, e.clone(), chain
+            e = torch.empty(0, dtype=torch.float32, device=device)
+            chain = torch.empty(self.n_timesteps + 1, 0, H, D, dtype=torch.float32, device=device) if return_chain else None
+            return torch.empty(0, H, D, dtype=torch.float32, device=device), e, e.clone(), chain
         kind = _FUSED_KINDS[sample_fn]
         keys = sorted(cond.keys())
         s = self._sampler(kind, B, H, keys, sample_kwargs, device, use_graph, skip_dead_evals)
@@ -467,7 +467,7 @@ class GaussianDiffusion(nn.Module):
                 thr = sample_kwargs.get('cost_threshold', 0)
                 s['thr'].copy_(torch.as_tensor(thr, device=device, dtype=torch.float32).expand(B))
         if return_chain and s['chain'] is None:
-            s['chain'] = torch.empty(self.n_timesteps + 1, B, H, D, device=device)
+            s['chain'] = torch.empty(self.n_timesteps + 1, B, H, D, dtype=torch.float32, device=device)
         chain = s['chain'] if return_chain else None
         bound = (s['noise'].data_ptr(), None if chain is None else chain.data_ptr())
         if s.get('bound') != bound:                 # set-up for this set of buffers: launch plans + graph capture
@@ -504,7 +504,7 @@ class GaussianDiffusion(nn.Module):
                 chain = chain.permute(1, 0, 2, 3).clone()                                # [B, T+1, H, D]
         else:
             draws = iter(noise) if noise is not None else None
-            x = next(draws).to(device).clone() if draws else torch.randn(shape, device=device)
+            x = next(draws).to(device).clone() if draws else torch.randn(shape, dtype=torch.float32, device=device)
             x = apply_conditioning(x, cond, self.action_dim)
             chain = [x] if return_chain else None
             for i in reversed(range(0, self.n_timesteps)):

@@ -218,7 +218,7 @@ class GuidedPolicy:
                                               B // sample_batch_size, _lib.ptr(order), st))
             index = order
         st_act = self._stats('actions', self.action_dim)
-        act_dev = torch.empty(index.numel(), self.action_dim, device=dev)
+        act_dev = torch.empty(index.numel(), self.action_dim, dtype=torch.float32, device=dev)
         _lib.check(lib.trebi_policy_first_action(
             ctx, _lib.ptr(x), B, H, dm.transition_dim, self.action_dim, _lib.ptr(index), index.numel(),
             _lib.ptr(st_act[0]) if st_act else None, _lib.ptr(st_act[1]) if st_act else None, _lib.ptr(act_dev), st))
@@ -243,7 +243,7 @@ class GuidedPolicy:
             if hasattr(thr, '__len__'):
                 thr = torch.tensor(np.asarray(thr, np.float32)).repeat(batch_size)
             else:
-                thr = torch.tensor([float(thr)]).repeat(batch_size)
+                thr = torch.tensor([float(thr)], dtype=torch.float32).repeat(batch_size)
             self.sample_kwargs['cost_threshold'] = thr.to(self.device)
         samples = self.diffusion_model(conditions, guide=self.guide, verbose=verbose, horizon=plan_horizon,
                                        sample_batch_size=sample_batch_size, **self.sample_kwargs)

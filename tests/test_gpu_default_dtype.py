@@ -98,3 +98,23 @@ def test_clipping_under_another_default_device():
     with default(device='cuda'):
         got = clip_once()
     same(want, got)
+
+
+def plan_once(diff, noise, chain):
+    from diffuser.models.diffusion import default_sample_fn
+    obs = torch.linspace(-1, 1, OBS, dtype=torch.float32, device='cuda')[None].repeat(4, 1)
+    out = diff.p_sample_loop((4, H, D), {0: obs}, sample_fn=default_sample_fn, verbose=False, noise=noise, return_chain=chain)
+    return [v.clone() for v in (out.trajectories, out.values, *([out.chains] if chain else []))]
+
+
+@pytest.mark.parametrize('dtype', ['float64', 'bfloat16', 'float16'])
+def test_planning_under_another_default_type(dtype):
+    from test_gpu_finetune import model
+    noise = torch.randn(T + 1, 4, H, D, dtype=torch.float32, generator=torch.Generator().manual_seed(3)).cuda()
+    diffs = [model()[0] for _ in range(2)]
+    for chain in (False, True):
+        want = plan_once(diffs[0], noise, chain)
+        with default(getattr(torch, dtype)):
+            got = plan_once(diffs[1], noise, chain)
+            assert diffs[1].p_sample_loop((0, H, D), {0: torch.zeros(0, OBS, dtype=torch.float32, device='cuda')}).trajectories.dtype == torch.float32
+        same(want, got)
