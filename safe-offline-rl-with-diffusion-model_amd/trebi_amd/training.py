@@ -38,6 +38,11 @@ def _flatten_into(module, names, flat):
     assert off == flat.numel()
 
 
+def _changes(v):
+    """How often a tensor was changed in place (tensors made in inference mode do not say)."""
+    return None if v.is_inference() else v._version
+
+
 class TrainEngine:
     """Flat parameter / gradient / Adam / EMA buffers + the library's trainer object for one GaussianDiffusion."""
 
@@ -145,7 +150,8 @@ class TrainEngine:
 
     # ---- fine-tuning: losses over the log-probabilities of denoise transitions (trebi_amd/losses.py) ----
     def forward(self, x, t):
-        """pred = unet(x, t) [B, H, D], with what backward() reads kept: B up to max_batch, x as the net is to see it."""
+        """pred = unet(x, t) [B, H, D], with what backward() reads kept: B up to max_batch, x as the net is to see it.  backward() reads
+        x and t again where they already are float32 / int64 and contiguous: not to be changed in place before it."""
         B = x.shape[0]
         if x.shape != (B, self.diffusion.horizon, self.diffusion.transition_dim) or t.shape != (B,):
             raise RuntimeError('x must be [batch, horizon, transition_dim] and t [batch]')
@@ -157,7 +163,7 @@ class TrainEngine:
         self._kept = None
         if B:
             _lib.check(_lib.lib().trebi_trainer_forward(self.h, _lib.ptr(x), _lib.ptr(t), _lib.ptr(pred), B, self._stream()))
-            self._kept = (x, t)                               # the backward reads them again
+            self._kept = (x, t, _changes(x), _changes(t))     # the backward reads them again
         return pred
 
     def backward(self, grad_pred):
@@ -166,7 +172,9 @@ class TrainEngine:
             return
         if getattr(self, '_kept', None) is None:
             raise RuntimeError('backward() follows forward(), once')
-        x, t = self._kept
+        x, t, *changes = self._kept
+        if changes != [_changes(x), _changes(t)]:
+            raise RuntimeError('x or t was changed in place since forward(); backward() reads them again')
         g = grad_pred.to(self.device, torch.float32).contiguous()
         if g.shape != x.shape:
             raise RuntimeError(f'grad_pred has shape {tuple(g.shape)}, the forward\'s output {tuple(x.shape)}')
