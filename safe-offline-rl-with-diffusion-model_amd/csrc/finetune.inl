@@ -5,23 +5,6 @@
 
 namespace {
 
-// The context's device for the length of a call; the caller's current device is put back.
-struct DeviceGuard {
-  int before = -1;
-  hipError_t err;
-  explicit DeviceGuard(int device) {
-    err = hipGetDevice(&before);
-    if (err == hipSuccess && before != device) err = hipSetDevice(device);
-    else if (err == hipSuccess) before = -1;
-  }
-  ~DeviceGuard() {
-    if (before >= 0) (void)hipSetDevice(before);
-  }
-};
-#define ON_DEVICE(ctx)                    \
-  DeviceGuard on_device((ctx)->device);   \
-  HIPCHK(on_device.err)
-
 size_t al256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Elements of a chunk.  Up to 8 M elements each workgroup gets one of 4096, whose loads are all in flight at once (bfloat16,

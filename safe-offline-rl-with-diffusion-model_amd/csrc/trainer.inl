@@ -298,7 +298,7 @@ extern "C" int trebi_trainer_create(trebi_ctx* ctx, const trebi_train_desc* desc
   if (!ctx || !out || max_batch < 1) return fail(TREBI_BAD_ARG, "null argument");
   trebi_net_desc nd;
   if (int e = trainer_net_desc(desc, &nd)) return e;
-  HIPCHK(hipSetDevice(ctx->device));
+  ON_DEVICE(ctx);
   HIPCHK(train_init_device());
   std::unique_ptr<trebi_trainer> tr(new trebi_trainer);
   tr->ctx = ctx; tr->d = *desc; tr->maxB = max_batch;
@@ -445,7 +445,7 @@ static int trainer_repack(trebi_trainer* tr, hipStream_t st) {
 
 extern "C" int trebi_trainer_repack(trebi_trainer* tr, void* stream) {
   if (!tr || !tr->bound) return fail(TREBI_BAD_ARG, "trainer is null or not bound");
-  HIPCHK(hipSetDevice(tr->ctx->device));
+  ON_DEVICE(tr->ctx);
   tr->fwd_x = nullptr;                             // a backward would run on other parameters than its forward
   return trainer_repack(tr, (hipStream_t)stream);
 }
@@ -455,7 +455,7 @@ extern "C" int trebi_trainer_bind(trebi_trainer* tr, float* params, float* grads
                                   const float* sqrt_one_minus_alphas_cumprod) {
   if (!tr || !params || !grads || !loss_weights || !sqrt_alphas_cumprod || !sqrt_one_minus_alphas_cumprod)
     return fail(TREBI_BAD_ARG, "null argument");
-  HIPCHK(hipSetDevice(tr->ctx->device));
+  ON_DEVICE(tr->ctx);
   HIPCHK(hipDeviceSynchronize());
   trebi_net* net = tr->net;
   const int H = tr->d.horizon, D = net->desc.transition_dim, T = tr->d.n_timesteps, dim = net->desc.dim;
@@ -540,6 +540,7 @@ extern "C" int trebi_trainer_bind(trebi_trainer* tr, float* params, float* grads
 
 extern "C" int trebi_trainer_set_precision(trebi_trainer* tr, int mode, int min_batch) {
   if (!tr) return fail(TREBI_BAD_ARG, "null trainer");
+  ON_DEVICE(tr->ctx);
   tr->fwd_x = nullptr;
   if (int e = trebi_net_set_precision(tr->net, mode, min_batch)) return e;
   if (tr->bound && mode == 1)
@@ -701,7 +702,7 @@ extern "C" int trebi_trainer_accumulate(trebi_trainer* tr, const float* x_start,
   if (B < 1 || B > tr->maxB) return fail(TREBI_BAD_SHAPE, "batch %d outside 1..%d (max_batch of trebi_trainer_create)", B, tr->maxB);
   if (tr->d.n_cond > 0 && !cond) return fail(TREBI_BAD_ARG, "cond is null");
   hipStream_t st = (hipStream_t)stream;
-  HIPCHK(hipSetDevice(tr->ctx->device));
+  ON_DEVICE(tr->ctx);
   trebi_net* net = tr->net;
   const trebi_train_desc& d = tr->d;
   const int H = d.horizon, D = net->desc.transition_dim, T = d.n_timesteps;
@@ -737,7 +738,7 @@ static int trainer_io(trebi_trainer* tr, const float* x, const int64_t* tsteps, 
 
 extern "C" int trebi_trainer_forward(trebi_trainer* tr, const float* x, const int64_t* tsteps, float* pred, int B, void* stream) {
   if (int e = trainer_io(tr, x, tsteps, pred, B)) return e;
-  HIPCHK(hipSetDevice(tr->ctx->device));
+  ON_DEVICE(tr->ctx);
   const std::vector<Tile>*tf, *tbw;
   if (int e = trainer_tiles(tr, B, &tf, &tbw)) return e;
   Resolver r{tr->net, tr->net->offsets(B), trainer_binding(tr, x, tsteps, pred, nullptr), B};
@@ -751,7 +752,7 @@ extern "C" int trebi_trainer_backward(trebi_trainer* tr, const float* x, const i
   if (int e = trainer_io(tr, x, tsteps, grad_pred, B)) return e;
   if (tr->fwd_x != x || tr->fwd_t != tsteps || tr->fwd_B != B)
     return fail(TREBI_BAD_ARG, "the last call on this trainer was not trebi_trainer_forward on the same x, t and batch");
-  HIPCHK(hipSetDevice(tr->ctx->device));
+  ON_DEVICE(tr->ctx);
   const std::vector<Tile>*tf, *tbw;
   if (int e = trainer_tiles(tr, B, &tf, &tbw)) return e;
   Resolver r{tr->net, tr->net->offsets(B), trainer_binding(tr, x, tsteps, nullptr, const_cast<float*>(grad_pred)), B};
@@ -766,7 +767,7 @@ static int trainer_step(trebi_trainer* tr, int64_t adam_step, float lr, float be
   if (adam_step < 1) return fail(TREBI_BAD_ARG, "adam_step counts from 1");
   if (ema_mode < 0 || ema_mode > 2 || (ema_mode && !tr->ema)) return fail(TREBI_BAD_ARG, "bad ema_mode / no EMA buffer bound");
   if (clip && !(max_norm >= 0.f)) return fail(TREBI_BAD_ARG, "max_norm must not be negative");
-  HIPCHK(hipSetDevice(tr->ctx->device));
+  ON_DEVICE(tr->ctx);
   tr->fwd_x = nullptr;
   const float* coef = nullptr;
   if (clip) {                                      // the norm and the factor; the Adam kernel scales as it reads

@@ -42,6 +42,23 @@ static int fail(int code, const char* fmt, ...) {
                   __FILE__, __LINE__);                                                        \
   } while (0)
 
+// The context's device for the length of a call; the caller's current device is put back.
+struct DeviceGuard {
+  int before = -1;
+  hipError_t err;
+  explicit DeviceGuard(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device) err = hipSetDevice(device);
+    else if (err == hipSuccess) before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+#define ON_DEVICE(ctx)                    \
+  DeviceGuard on_device((ctx)->device);   \
+  HIPCHK(on_device.err)
+
 struct Unsupported {
   std::string msg;
 };
@@ -1734,7 +1751,8 @@ extern "C" int trebi_ctx_create(int device, trebi_ctx** out) {
   int n = 0;
   HIPCHK(hipGetDeviceCount(&n));
   if (device < 0 || device >= n) return fail(TREBI_BAD_ARG, "device %d out of range (%d visible)", device, n);
-  HIPCHK(hipSetDevice(device));
+  DeviceGuard on_device(device);
+  HIPCHK(on_device.err);
   hipDeviceProp_t prop;
   HIPCHK(hipGetDeviceProperties(&prop, device));
   if (std::string(prop.gcnArchName).rfind("gfx950", 0) != 0)
