@@ -262,32 +262,23 @@ __device__ __forceinline__ RowsOfPack rows_packed(const PolicyP& p, Window& w, l
     q.valid = low_bits(N);
     return q;
   }
-  if (i >= t.n) i = t.n - 1;                                           // (a lane behind the end: its answer is not used)
-  int row;
-  long long s, e, e2;
-  if (w.r + 61 < rows && (long long)__builtin_amdgcn_readlane(w.at, 61) <= lw) {       // more sequences than lanes
-    row = find_row(t.cu, w.r, rows - 1, i);
-    row_bounds(t, row, &s, &e);
-    e2 = e;
-    if (row + 1 < rows) {
-      long long s2;
-      row_bounds(t, row + 1, &s2, &e2);
-    }
-  } else {
-    int pos = 0;
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1)
-      if ((long long)__shfl(w.at, pos + step, 64) <= i) pos += step;
-    pos = min(pos, min(rows - 1 - w.r, 61));
-    q.pos = pos;
-    row = w.r + pos;
-    s = __shfl(w.at, pos, 64);
-    e = __shfl(w.at, pos + 1, 64);
-    e2 = __shfl(w.at, pos + 2, 64);
-    s = s < 0 ? 0 : (s > t.n ? t.n : s);
-    e = e < s ? s : (e > t.n ? t.n : e);
-    e2 = e2 < e ? e : (e2 > t.n ? t.n : e2);
+  if (w.r + 61 < rows && (long long)__builtin_amdgcn_readlane(w.at, 61) <= lw) {       // more sequences than lanes: the caller's policy_rest
+    q.k1 = 0;
+    q.valid = 0u;
+    return q;
   }
+  if (i >= t.n) i = t.n - 1;                                           // (a lane behind the end: its answer is not used)
+  int pos = 0;
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1)
+    if ((long long)__shfl(w.at, pos + step, 64) <= i) pos += step;
+  pos = min(pos, min(rows - 1 - w.r, 61));
+  q.pos = pos;
+  const int row = w.r + pos;
+  long long s = __shfl(w.at, pos, 64), e = __shfl(w.at, pos + 1, 64), e2 = __shfl(w.at, pos + 2, 64);
+  s = s < 0 ? 0 : (s > t.n ? t.n : s);
+  e = e < s ? s : (e > t.n ? t.n : e);
+  e2 = e2 < e ? e : (e2 > t.n ? t.n : e2);
   const bool two = e < i + N && row + 1 < rows;
   q.single = i < s || (two && e2 < i + N && row + 2 < rows);
   q.k1 = e <= i ? 0 : e - i < N ? (int)(e - i) : N;
