@@ -384,12 +384,12 @@ __device__ __forceinline__ void policy_pack(const PolicyP& p, const Window& w, l
     done = p.fdual == INFINITY ? policy_row<T, KL, TA, N, false>(p, x, q.a, W, g, a) : policy_row<T, KL, TA, N, true>(p, x, q.a, W, g, a);
     if (!done) a = PolicyAcc{0, 0, 0, 0};
   }
-  auto token = [&](int k, float A, float u) {         // where tokens may not count: their values are replaced, e^0 taken back
+  auto token = [&](int k, float A, float u) {         // where tokens may not count: their values are replaced, their e^0 is left out
     const bool on = (q.valid >> k) & 1u;
     const float l = on ? x.l.at(k) : 0.f, o = on ? x.o.at(k) : 0.f, f = KL && on ? x.f.at(k) : 0.f;
     const float t = TA ? x.a.at(k) : A, At = on ? t : 0.f, ut = on ? u : 0.f;
-    const float d = policy_token<KL>(p, l, o, f, At, ut, k, a);
-    if (!on) a.rho -= 1.f;
+    const float rho = a.rho, d = policy_token<KL>(p, l, o, f, At, ut, k, a);
+    a.rho = on ? a.rho : rho;
     return on ? W * ut * d : 0.f;
   };
   if (PACKED && !done && !q.one_row && __any(q.single)) {    // some lane's tokens lie in more than two sequences: all look each token up
