@@ -25,9 +25,11 @@ namespace trebi {
 // border's own float32 value but can make the two equal; only then the comparison is made again in float64, where the
 // difference is exact for every input type.
 // ---------------------------------------------------------------------------------------------------------------
-// (pg in float64 from the token on: many tokens of a row are held at the same border, and float32 sums of the same few values
-// round the same way again and again -- 3e-9 of a mean ratio, which a sum over advantages of both signs does not hide)
-struct PolicyAcc { double pg; float kl, rho; unsigned cut; };
+// Sums are float64 from the token on: many tokens are held at the same border, or hold the same ratio, and float32 sums of the same
+// few values round the same way again and again (9e-8 of eight equal terms, which advantages of both signs do not hide).
+struct PolicySum { double pg, kl, rho; unsigned cut, cnt; };      // (a thread has fewer than 2^31 of 2^46 tokens)
+// A token: its gradient before its weight, KL term, ratio, the ratio that its loss takes, and whether that is a border's
+struct PolicyToken { float g, kl, rho, used; bool cut; };
 
 // e^x by the exponential unit: within (|x| + 2) 2^-24 of e^x, which the rounding of the difference x (|x| 2^-24) allows for
 __device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
@@ -73,28 +75,31 @@ __device__ __forceinline__ bool beyond(const PolicyP& p, float lp, float old, fl
   return over || far || under;
 }
 
-// One token.  Returns the gradient before its weight; bit `e` of a.cut says whether it is beyond a border.
 template <int KL>
-__device__ __forceinline__ float policy_token(const PolicyP& p, float lp, float old, float ref, float A, float u, int e, PolicyAcc& a) {
+__device__ __forceinline__ PolicyToken policy_token(const PolicyP& p, float lp, float old, float ref, float A) {
   // (by value: a selection between fields of the kernel's arguments would be one of addresses, and put them into scratch)
   const float fhi = p.fhi, flo = p.flo, fdual = p.fdual, vhi = p.vhi, vlo = p.vlo, vdual = p.vdual;
   const float d = lp - old;
   float held = A > 0.f ? vhi : (d > 0.f ? vdual : vlo);
-  bool cut = A > 0.f ? d > fhi : (A < 0.f && (d < flo || d > fdual));
-  if (d == fhi || d == flo || d == fdual) cut = beyond(p, lp, old, A, &held);
-  const float rho = exp_near(d);
-  const float pg = -A * (cut ? held : rho);
-  float g = cut ? 0.f : pg;
+  PolicyToken q;
+  q.cut = A > 0.f ? d > fhi : (A < 0.f && (d < flo || d > fdual));
+  if (d == fhi || d == flo || d == fdual) q.cut = beyond(p, lp, old, A, &held);
+  q.rho = exp_near(d);
+  q.used = q.cut ? held : q.rho;
+  q.g = q.cut ? 0.f : -A * q.rho;
+  q.kl = 0.f;
   if (KL) {
-    float kl, dk;
-    kl_term<KL>(ref - lp, &kl, &dk);
-    g = fmaf(p.kl_coef, dk, g);
-    a.kl = fmaf(u, kl, a.kl);
+    float dk;
+    kl_term<KL>(ref - lp, &q.kl, &dk);
+    q.g = fmaf(p.kl_coef, dk, q.g);
   }
-  a.pg += (double)(u * pg);
-  a.rho += rho;
-  a.cut |= cut ? 1u << e : 0u;
-  return g;
+  return q;
+}
+// A token's terms, u: 1 / its row's length
+__device__ __forceinline__ void add_token(PolicySum& sum, const PolicyToken& q, float A, float u) {
+  sum.pg = fma(-(double)A * (double)u, (double)q.used, sum.pg);
+  sum.kl = fma((double)u, (double)q.kl, sum.kl);
+  sum.rho += (double)q.rho;
 }
 
 // What multiplies a token besides 1 / (its row's length): 1 / tokens, 1 / sequences or 1 / denominator.
@@ -174,8 +179,6 @@ __device__ __forceinline__ RowInfo row_info(const PolicyP& p, long long r, long 
   return ri;
 }
 
-struct PolicySum { double pg, kl, rho; long long cut, cnt; };
-
 __device__ __forceinline__ long long row_of(const TokenP& t, long long i) {
   return t.n <= 0xffffffffll ? (long long)((unsigned)i / (unsigned)t.len) : i / t.len;
 }
@@ -202,14 +205,11 @@ __device__ __forceinline__ void policy_one(const PolicyP& p, long long i, float 
     const float old = p.old ? load_one((const T*)p.old + k * p.ors + c * p.ocs) : lp;
     const float ref = p.ref ? load_one((const T*)p.ref + k * p.rrs + c * p.rcs) : 0.f;
     const float A = p.acs ? p.adv[k * p.ars + c * p.acs] : ri.A;
-    PolicyAcc a{0, 0, 0, 0};
-    g = !p.ref ? policy_token<0>(p, lp, old, ref, A, ri.u, 0, a) : p.kl == 1 ? policy_token<1>(p, lp, old, ref, A, ri.u, 0, a)
-      : p.kl == 2 ? policy_token<2>(p, lp, old, ref, A, ri.u, 0, a) : policy_token<3>(p, lp, old, ref, A, ri.u, 0, a);
-    g *= W * ri.u;
-    sum.pg += a.pg;
-    sum.kl += (double)a.kl;
-    sum.rho += (double)a.rho;
-    sum.cut += a.cut;
+    const PolicyToken q = !p.ref ? policy_token<0>(p, lp, old, ref, A) : p.kl == 1 ? policy_token<1>(p, lp, old, ref, A)
+                          : p.kl == 2 ? policy_token<2>(p, lp, old, ref, A) : policy_token<3>(p, lp, old, ref, A);
+    g = q.g * (W * ri.u);
+    add_token(sum, q, A, ri.u);
+    sum.cut += q.cut;
     sum.cnt += 1;
   }
   if (p.grad) store_one((T*)p.grad + i, g);
@@ -324,77 +324,93 @@ __device__ __forceinline__ RowsOfPack rows_padded(const PolicyP& p, long long i,
   return q;
 }
 
-// N tokens of one row that all count, in every lane.  With s the advantage's sign a token is beyond the border where s d
-// exceeds one number (and with a dual border where -s d, s < 0, exceeds another), and what the row shares is taken out of
-// the sums.  False: some lane's rounded difference equals a border, nothing was done.
+// With s the advantage's sign a token is beyond the border where s d exceeds one number (and with a dual border where -s d,
+// s < 0, exceeds another).
+struct Border { float at, held; };
+__device__ __forceinline__ Border border_of(const PolicyP& p, float A) {
+  const float fhi = p.fhi, flo = p.flo, vhi = p.vhi, vlo = p.vlo;
+  return {A > 0.f ? fhi : (A < 0.f ? -flo : INFINITY), A > 0.f ? vhi : vlo};
+}
+__device__ __forceinline__ float signed_by(float d, float A) { return __uint_as_float(__float_as_uint(d) ^ (__float_as_uint(A) & 0x80000000u)); }
+
+// Does a rounded difference of the wave's tokens equal a border?
 template <typename T, int KL, bool TA, int N, bool DUAL>
-__device__ __forceinline__ bool policy_row(const PolicyP& p, const PolicyLoad<T, KL, TA, N>& x, RowInfo row, float W, float* g, PolicyAcc& a) {
-  const float w = W * row.u, wk = w * p.kl_coef, fhi = p.fhi, flo = p.flo, fdual = p.fdual, vhi = p.vhi, vlo = p.vlo, vdual = p.vdual;
-  double reff = 0.0;
-  float rta = 0.f, kl = 0.f;
+__device__ __forceinline__ bool at_border(const PolicyP& p, const PolicyLoad<T, KL, TA, N>& x, float rowA) {
+  const float fdual = p.fdual;
   bool same = false;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float A = TA ? x.a.at(k) : rowA, d = x.l.at(k) - x.o.at(k);
+    same = same || signed_by(d, A) == border_of(p, A).at || (DUAL && d == fdual);
+  }
+  return __any(same);
+}
+
+// N tokens of one row that all count, none of them at a border, in every lane: what the row shares is taken out of the sums.
+template <typename T, int KL, bool TA, int N, bool DUAL>
+__device__ __forceinline__ void policy_row(const PolicyP& p, const PolicyLoad<T, KL, TA, N>& x, RowInfo row, float W, float* g, PolicySum& sum) {
+  const float w = W * row.u, wk = w * p.kl_coef, fdual = p.fdual, vdual = p.vdual;
+  double used = 0.0, rhos = 0.0, kl = 0.0;
   unsigned cuts = 0;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const float A = TA ? x.a.at(k) : row.A;
-    const float border = A > 0.f ? fhi : (A < 0.f ? -flo : INFINITY), held = A > 0.f ? vhi : vlo;
-    const float l = x.l.at(k), d = l - x.o.at(k);
-    const float sd = __uint_as_float(__float_as_uint(d) ^ (__float_as_uint(A) & 0x80000000u));
-    bool cut = sd > border;
-    same = same || sd == border;
-    const float rho = exp_near(d);
-    float r = cut ? held : rho, live = cut ? 0.f : rho;
+    const Border b = border_of(p, A);
+    const float l = x.l.at(k), d = l - x.o.at(k), rho = exp_near(d);
+    bool cut = signed_by(d, A) > b.at;
+    float r = cut ? b.held : rho, live = cut ? 0.f : rho;
     if (DUAL) {
       const bool far = A < 0.f && d > fdual;
-      same = same || d == fdual;
       r = far ? vdual : r;
       live = far ? 0.f : live;
       cut = cut || far;
     }
-    cuts += cut ? 1u : 0u;
-    a.rho += rho;
+    cuts += cut;
+    rhos += (double)rho;
     if (TA) {
-      rta = fmaf(-A, r, rta);
+      used = fma(-(double)A, (double)r, used);
       g[k] = -A * live * w;
     } else {
-      reff += (double)r;
+      used += (double)r;
       g[k] = (-row.A * w) * live;
     }
     if (KL) {
       float q, dk;
       kl_term<KL>(x.f.at(k) - l, &q, &dk);
-      kl += q;
+      kl += (double)q;
       g[k] = fmaf(wk, dk, g[k]);
     }
   }
-  a.pg = TA ? (double)(row.u * rta) : (double)(-row.A * row.u) * reff;
-  a.kl = row.u * kl;
-  a.cut = (1u << cuts) - 1u;                          // (as many bits as tokens beyond a border)
-  return !__any(same);
+  const double u = (double)row.u;
+  sum.pg = fma(TA ? u : -(double)row.A * u, used, sum.pg);
+  if (KL) sum.kl = fma(u, kl, sum.kl);
+  sum.rho += rhos;
+  sum.cut += cuts;
+  sum.cnt += N;
 }
 
 // A thread's N tokens from i on, loaded into x, of the rows q; `mine`: they are all there.  All lanes active.
-template <typename T, int KL, bool TA, bool PACKED, int N>
+template <typename T, int KL, bool TA, bool PACKED, int N, bool DUAL>
 __device__ __forceinline__ void policy_pack(const PolicyP& p, const Window& w, long long i, const PolicyLoad<T, KL, TA, N>& x, RowsOfPack q,
                                             unsigned masked, bool mine, float W, PolicySum& sum) {
-  PolicyAcc a{0, 0, 0, 0};
   float g[N];
-  bool done = __all(q.valid == low_bits(N)) && q.one_row;
-  if (done) {
-    done = p.fdual == INFINITY ? policy_row<T, KL, TA, N, false>(p, x, q.a, W, g, a) : policy_row<T, KL, TA, N, true>(p, x, q.a, W, g, a);
-    if (!done) a = PolicyAcc{0, 0, 0, 0};
-  }
-  auto token = [&](int k, float A, float u) {         // where tokens may not count: their values are replaced, their e^0 is left out
-    const bool on = (q.valid >> k) & 1u;
+  const bool row = __all(q.valid == low_bits(N)) && q.one_row && !at_border<T, KL, TA, N, DUAL>(p, x, q.a.A);
+  auto token = [&](int k, bool on, float A, float u) {     // where tokens may not count: their values are replaced, their e^0 is left out
     const float l = on ? x.l.at(k) : 0.f, o = on ? x.o.at(k) : 0.f, f = KL && on ? x.f.at(k) : 0.f;
     const float t = TA ? x.a.at(k) : A, At = on ? t : 0.f, ut = on ? u : 0.f;
-    const float rho = a.rho, d = policy_token<KL>(p, l, o, f, At, ut, k, a);
-    a.rho = on ? a.rho : rho;
-    return on ? W * ut * d : 0.f;
+    PolicyToken v = policy_token<KL>(p, l, o, f, At);
+    v.rho = on ? v.rho : 0.f;
+    add_token(sum, v, At, ut);
+    sum.cut += on && v.cut;
+    sum.cnt += on;
+    g[k] = on ? W * ut * v.g : 0.f;
+    // one token after the other: all of them side by side do not fit the registers (scratch in every 16-bit kernel)
+    asm volatile("" : "+v"(sum.pg), "+v"(sum.kl), "+v"(sum.rho), "+v"(g[k]));
   };
-  if (PACKED && !done && !q.one_row && __any(q.single)) {    // some lane's tokens lie in more than two sequences: all look each token up
+  if (row) {
+    policy_row<T, KL, TA, N, DUAL>(p, x, q.a, W, g, sum);
+  } else if (PACKED && !q.one_row && __any(q.single)) {    // some lane's tokens lie in more than two sequences: all look each token up
     int pos = q.pos;
-    q.valid = 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       for (;;) {                                      // past the sequences that end here (empty ones too)
@@ -406,21 +422,13 @@ __device__ __forceinline__ void policy_pack(const PolicyP& p, const Window& w, l
       long long s = __shfl(w.at, pos, 64), e = __shfl(w.at, pos + 1, 64);
       s = s < 0 ? 0 : (s > p.tk.n ? p.tk.n : s);
       e = e < s ? s : (e > p.tk.n ? p.tk.n : e);
-      q.valid |= mine && i + k >= s && i + k < e ? masked & (1u << k) : 0u;
       const RowInfo ri = row_info(p, w.r + pos, e - s);
-      g[k] = token(k, ri.A, ri.u);
+      token(k, mine && i + k >= s && i + k < e && (masked & (1u << k)), ri.A, ri.u);
     }
-    a.cut &= q.valid;
-  } else if (!done) {
+  } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) g[k] = token(k, k < q.k1 ? q.a.A : q.b.A, k < q.k1 ? q.a.u : q.b.u);
-    a.cut &= q.valid;
+    for (int k = 0; k < N; ++k) token(k, (q.valid >> k) & 1u, k < q.k1 ? q.a.A : q.b.A, k < q.k1 ? q.a.u : q.b.u);
   }
-  sum.pg += a.pg;
-  if (KL) sum.kl += (double)a.kl;
-  sum.rho += (double)a.rho;
-  sum.cut += __popc(a.cut);
-  sum.cnt += __popc(q.valid);
   if (p.grad && mine) store_vec<N>((T*)p.grad + i, g);
 }
 
@@ -440,7 +448,7 @@ __device__ __forceinline__ void policy_rest(const PolicyP& p, const Window& w, b
 
 // Tokens [begin, end) of flat tensors by a workgroup.  Where a mask or lengths say which tokens count, the loads wait for
 // that (p.early: not in calls of one turn, which latency bounds).
-template <typename T, int KL, bool TA, bool PACKED>
+template <typename T, int KL, bool TA, bool PACKED, bool DUAL>
 __device__ __forceinline__ void policy_flat(const PolicyP& p, long long begin, long long end, float W, PolicySum& sum) {
   constexpr int N = 16 / (int)sizeof(T);
   Window win{-1, 0};
@@ -469,7 +477,7 @@ __device__ __forceinline__ void policy_flat(const PolicyP& p, long long begin, l
     }
     if (!p.early && (q.valid || q.single)) x.load(p, i);
     if (__any(q.valid || q.single)) {
-      policy_pack<T, KL, TA, PACKED, N>(p, win, i, x, q, masked, whole, W, sum);
+      policy_pack<T, KL, TA, PACKED, N, DUAL>(p, win, i, x, q, masked, whole, W, sum);
     } else if (p.grad && whole) {                     // a wave of tokens that do not count
       const float zero[N] = {};
       store_vec<N>((T*)p.grad + i, zero);
@@ -480,7 +488,7 @@ __device__ __forceinline__ void policy_flat(const PolicyP& p, long long begin, l
 
 // The same for packed sequences without a mask: the loads of a turn go out before the turn before it is computed, and
 // without a condition (past the end: the last tokens again), so that nothing waits for them but their own use.
-template <typename T, int KL, bool TA>
+template <typename T, int KL, bool TA, bool DUAL>
 __device__ __forceinline__ void policy_stream(const PolicyP& p, long long begin, long long end, float W, PolicySum& sum) {
   constexpr int N = 16 / (int)sizeof(T);
   Window win{-1, 0};
@@ -497,7 +505,7 @@ __device__ __forceinline__ void policy_stream(const PolicyP& p, long long begin,
       if (q.one_row || q.pos >= 0) {
         if (!whole) q.valid = 0u;
         q.single = q.single && whole;
-        policy_pack<T, KL, TA, true, N>(p, win, i, x, q, low_bits(N), whole, W, sum);
+        policy_pack<T, KL, TA, true, N, DUAL>(p, win, i, x, q, low_bits(N), whole, W, sum);
         if ((lw + 1 - iw) % N) policy_rest<T, N>(p, win, false, i, iw, lw, W, sum);
       } else {
         policy_rest<T, N>(p, win, true, i, iw, lw, W, sum);
@@ -507,10 +515,11 @@ __device__ __forceinline__ void policy_stream(const PolicyP& p, long long begin,
   }
 }
 
-// KIND 0: any strides, token by token; 1: flat padded rows; 2: packed; 3: packed with a mask.  Waves on a SIMD: 5 where the
-// registers allow it without spilling (4096 x 8192 bfloat16: 58 us, with 4: 70), 4 for the others (512 x 2047 with the
-// third KL term: 9 us, with 5: 12; packed: 29 against 35)
-template <typename T, int KL, bool TA, int KIND>
+// KIND 0: any strides, token by token; 1: flat padded rows; 2: packed; 3: packed with a mask.  DUAL: is there a dual border (decided
+// inside the kernel it costs the registers of both).  Waves on a SIMD: 5 where that pays (4096 x 8192 bfloat16, second KL term: 63 us,
+// with 4: 76), 4 for the others (packed, masked, bfloat16, third KL term, an advantage a token: 28 us, with 5: 31; 512 x 2047: 14.8 and
+// 15.1).  No instance spills vector registers.
+template <typename T, int KL, bool TA, int KIND, bool DUAL>
 __global__ __launch_bounds__(256, KIND == 1 && !TA && KL < 3 ? 5 : 4) void policy_kernel(PolicyP p) {
   __shared__ double lds[5 * LOSS_VALS];
   const double W = policy_weight_parts(p, lds);
@@ -520,8 +529,8 @@ __global__ __launch_bounds__(256, KIND == 1 && !TA && KL < 3 ? 5 : 4) void polic
   if (KIND == 0) {
     for (long long i = begin + threadIdx.x; i < end; i += 256) policy_one<T>(p, i, Wg, sum);
   } else {
-    if constexpr (KIND == 2) policy_stream<T, KL, TA>(p, begin, end, Wg, sum);
-    else policy_flat<T, KL, TA, KIND == 3>(p, begin, end, Wg, sum);
+    if constexpr (KIND == 2) policy_stream<T, KL, TA, DUAL>(p, begin, end, Wg, sum);
+    else policy_flat<T, KL, TA, KIND == 3, DUAL>(p, begin, end, Wg, sum);
   }
   if (blockIdx.x == 0 && threadIdx.x == 0 && gridDim.x > 1) *p.weight = W;
   double acc[LOSS_VALS] = {sum.pg, sum.kl, (double)sum.cut, sum.rho, (double)sum.cnt};
@@ -536,7 +545,11 @@ __global__ __launch_bounds__(256, KIND == 1 && !TA && KL < 3 ? 5 : 4) void polic
 
 template <typename T, int KL>
 static hipError_t launch_policy_k(const PolicyP& p, int blocks, hipStream_t st) {
-#define GO(TA, KIND) hipLaunchKernelGGL((policy_kernel<T, KL, TA, KIND>), dim3(blocks), dim3(256), 0, st, p)
+#define GO(TA, KIND)                                                                                                              \
+  do {                                                                                                                            \
+    if (p.dual < INFINITY) hipLaunchKernelGGL((policy_kernel<T, KL, TA, KIND, true>), dim3(blocks), dim3(256), 0, st, p);         \
+    else hipLaunchKernelGGL((policy_kernel<T, KL, TA, KIND, false>), dim3(blocks), dim3(256), 0, st, p);                          \
+  } while (0)
   if (!p.tk.packed) { if (p.acs) GO(true, 1); else GO(false, 1); }
   else if (!p.tk.mask) { if (p.acs) GO(true, 2); else GO(false, 2); }
   else { if (p.acs) GO(true, 3); else GO(false, 3); }
@@ -545,7 +558,7 @@ static hipError_t launch_policy_k(const PolicyP& p, int blocks, hipStream_t st) 
 template <typename T>
 static hipError_t launch_policy_t(const PolicyP& p, int blocks, hipStream_t st) {
   if (!p.flat) {
-    hipLaunchKernelGGL((policy_kernel<T, 0, false, 0>), dim3(blocks), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((policy_kernel<T, 0, false, 0, true>), dim3(blocks), dim3(256), 0, st, p);
     return hipGetLastError();
   }
   switch (p.ref ? p.kl : 0) {
