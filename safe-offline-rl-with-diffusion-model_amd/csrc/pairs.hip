@@ -31,11 +31,11 @@ __device__ __forceinline__ PairOut pair_math(const PairP& p, long long k, double
   const double h = dc - dr, z = p.beta * h - p.margin;
   double slope;
   if (p.kind == 0) {
-    const float q = expf(-fabsf((float)z)), l1 = log1pf(q), inv = 1.f / (1.f + q);
-    const float big = inv, small = q * inv;                              // sigmoid(|z|), sigmoid(-|z|)
-    const double pos = (double)l1 + (z < 0 ? -z : 0.0), neg = (double)l1 + (z > 0 ? z : 0.0);   // softplus(-z), softplus(z)
+    // (in float64: a float32 argument of the exponential, off by |z| 2^-24, would make loss and slope of decided pairs as far off)
+    const double q = exp(-fabs(z)), l1 = log1p(q), big = 1.0 / (1.0 + q), small = q * big;      // sigmoid(|z|), sigmoid(-|z|)
+    const double pos = l1 + (z < 0 ? -z : 0.0), neg = l1 + (z > 0 ? z : 0.0);                   // softplus(-z), softplus(z)
     o.loss = (1.0 - (double)p.smooth) * pos + (p.smooth > 0.f ? (double)p.smooth * neg : 0.0);
-    const float sn = z >= 0 ? small : big, sp = z >= 0 ? big : small;    // sigmoid(-z), sigmoid(z)
+    const double sn = z >= 0 ? small : big, sp = z >= 0 ? big : small;                          // sigmoid(-z), sigmoid(z)
     slope = p.beta * ((double)p.smooth * sp - (1.0 - (double)p.smooth) * sn);
     if (z != z) { o.loss = z; slope = z; }
   } else if (p.kind == 1) {

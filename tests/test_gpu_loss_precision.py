@@ -1,5 +1,5 @@
 """GPU: how exact the fine-tuning losses are where errors do not average out: sums of many equal terms, means over few tokens among
-many that do not count, tokens exactly at a border."""
+many that do not count, tokens exactly at a border, pairs far from the middle."""
 import math
 
 import numpy as np
@@ -141,3 +141,25 @@ def test_single_tokens_at_each_border_of_whole_rows(layout, adv, dual):
     g = np64(got.grad).reshape(R, L)[np.arange(R), at]
     wg = np.array([want[5][r][at[r]] for r in range(R)])
     assert ((g == 0) == (wg == 0)).all()
+
+
+# ------------------------------------------------------------------------------------------------- far from the middle
+def test_preference_loss_and_slope_of_decided_pairs():
+    """The loss of a pair z > 0 apart is log(1 + e^-z) and its slope -sigmoid(-z): small numbers, right to the float32 they are
+    returned in (everything before is float64; two roundings allowed), where z itself is not a float32 number too."""
+    from trebi_amd.losses import preference_loss
+    for margin in (0.0, 0.1, 1e-7):
+        for c, r in ((0.0, -2.0), (-1.0, -6.1), (0.0, -20.0), (-0.3, -40.7), (-3.0, -83.0), (-20.0, -0.7), (-80.3, -1.0)):
+            lp = torch.tensor([[c], [r]])
+            z = float(lp[0, 0]) - float(lp[1, 0]) - float(np.float32(margin))
+            got = preference_loss(lp.cuda(), beta=1.0, margin=margin)
+            loss = math.log1p(math.exp(-abs(z))) + max(-z, 0.0)
+            slope = 1 / (1 + math.exp(z))
+            assert abs(float(got.loss) - loss) <= 2 * F.F24 * loss, (c, r, margin)
+            assert abs(float(got.grad[0, 0]) + slope) <= 2 * F.F24 * slope and abs(float(got.grad[1, 0]) - slope) <= 2 * F.F24 * slope, (c, r, margin)
+            e = float(np.float32(0.1))
+            got = preference_loss(lp.cuda(), beta=1.0, margin=margin, label_smoothing=0.1)
+            other = math.log1p(math.exp(-abs(z))) + max(z, 0.0)
+            loss, sl = (1 - e) * loss + e * other, e / (1 + math.exp(-z)) - (1 - e) * slope
+            assert abs(float(got.loss) - loss) <= 2 * F.F24 * loss
+            assert abs(float(got.grad[0, 0]) - sl) <= 2 * F.F24 * abs(sl) + 2.0 ** -50
