@@ -31,8 +31,9 @@ struct PolicySum { double pg, kl, rho; unsigned cut, cnt; };      // (a thread h
 // A token: its gradient before its weight, KL term, ratio, the ratio that its loss takes, and whether that is a border's
 struct PolicyToken { float g, kl, rho, used; bool cut; };
 
-// e^x by the exponential unit: within (|x| + 2) 2^-24 of e^x, which the rounding of the difference x (|x| 2^-24) allows for
-__device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+// e^x by the exponential unit, log2(e) in two parts: within (|x| + 2) 2^-24 of e^x, which the rounding of the difference x (|x| 2^-24)
+// allows for.  Results below 2^-126 may be 0.
+__device__ __forceinline__ float exp_near(float x) { return __builtin_amdgcn_exp2f(fmaf(x, 1.44269502f, x * 1.92596299e-8f)); }
 
 // e^x - 1 and e^x - x - 1 without cancellation: the series below |x| = 1 (its 12th term is under 2^-24 of the sum)
 __device__ __forceinline__ void exp_parts(float x, float* em1, float* rest) {

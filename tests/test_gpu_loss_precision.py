@@ -163,3 +163,23 @@ def test_preference_loss_and_slope_of_decided_pairs():
             loss, sl = (1 - e) * loss + e * other, e / (1 + math.exp(-z)) - (1 - e) * slope
             assert abs(float(got.loss) - loss) <= 2 * F.F24 * loss
             assert abs(float(got.grad[0, 0]) - sl) <= 2 * F.F24 * abs(sl) + 2.0 ** -50
+
+
+# ------------------------------------------------------------------------------------------------- the ratio itself
+@pytest.mark.parametrize('adv', ['row', 'token'])
+def test_every_ratio_is_within_its_bound(adv):
+    """With advantages of -+1, weight 1 and no old log-probability but 0, a token's gradient is +- its ratio, unrounded: e^x within
+    (|x| + 2) 2^-24 (the exponential's argument rounded in base 2, one step of the exponential unit).  Arguments just above a power
+    of two in base 2, where that rounding is largest."""
+    from trebi_amd.losses import policy_loss
+    rng = np.random.default_rng(0)
+    L = 8192
+    for k in range(-1, 7):
+        x = (math.log(2) * 2.0 ** k * (1 + 0.06 * rng.random((2, L)))).astype(np.float32)
+        x[1] *= -1
+        A = torch.tensor([-1.0, 1.0], device='cuda')            # no border holds ratios above 1 here, nor those below 1 there
+        lp = torch.from_numpy(x).cuda()
+        r = policy_loss(lp, A if adv == 'row' else A[:, None].expand(2, L).contiguous(), torch.zeros_like(lp), denominator=1.0)
+        got, want = np.abs(np64(r.grad)), np.exp(x.astype(np.float64))
+        assert float(r.clip_fraction) == 0.0
+        assert (np.abs(got / want - 1) <= (np.abs(x) + 2) * F.F24).all(), (k, np.abs(got / want - 1).max() / F.F24)
