@@ -56,6 +56,7 @@ class GradClipper:
         self.set = _lib.GradSet()
         _lib.check(lib.trebi_grad_set_fill(n, ptrs, numels, dtypes, _lib.ptr(host), nbytes, C.byref(self.set)))
         self.table = host.to(self.device)
+        self._made_on = _lib.stream(self.device)
         self._spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.tensors]
         self.total = int(self.set.total)
         self._ws_bytes = lib.trebi_grad_workspace_bytes(C.byref(self.set))
@@ -63,8 +64,10 @@ class GradClipper:
 
     def _buffers(self):
         """A workspace of this call's own (two calls may run at once), the norm, the stream."""
-        ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
-        return ws, torch.empty((), dtype=torch.float32, device=self.device), _lib.stream(self.device)
+        ws, st = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device), _lib.stream(self.device)
+        if st != self._made_on:                             # the table's memory waits for this stream before it serves others
+            self.table.record_stream(torch.cuda.current_stream(self.device))
+        return ws, torch.empty((), dtype=torch.float32, device=self.device), st
 
     def norm(self, grad_scale=1.0):
         """grad_scale * the norm, a device scalar."""
