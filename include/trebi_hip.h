@@ -423,7 +423,8 @@ int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens, const treb
 /* Preference loss over pairs of rows (row k < rows/2 is preferred to row k + rows/2), and its gradient:
  *   D_r = sum over the row's valid tokens of logp - ref (ref null: logp), with `average` divided by their number
  *   h = D_chosen - D_rejected,  z = beta h - margin
- *   l = (1 - e) softplus(-z) + e softplus(z) | max(0, 1 - z) | (z / beta - 1 / (2 beta))^2   (kind 0 | 1 | 2; e: smoothing)
+ *   l = (1 - e) softplus(-z) + e softplus(z) | max(0, 1 - z) | (z / beta - 1 / (2 beta))^2   (kind 0 | 1 | 2; e: label_smoothing,
+ *       which kinds 1 and 2 do not look at)
  *   loss = sum weights l / denominator (0: the number of pairs); a pair with an empty row gives nothing
  * grad: like the policy loss.  chosen_reward / rejected_reward: dev [rows/2], beta D.  stats: dev [3] loss, share of the
  * pairs that count with h > 0, their mean z. */

@@ -81,11 +81,11 @@ int token_args(const trebi_token_desc& d, TokenP* t) {
 }
 
 // One workgroup does it all up to 4096 tokens (at most 4 turns): calls of this size wait for their launches.  4096 float32 tokens
-// with lengths, enqueued one by one: 14 us, with three launches 20 (replayed from a graph 10.5 and 10.4); 8192, replayed: 17.5 and 10.8.
+// with lengths, enqueued one by one: 13.6 us, with two launches 17.6 (replayed from a graph 10.8 and 8.6); 8192: 18.2 and 17.7 (18.3 and 8.7).
 // policy workspace: partial counts, partial sums, a count for each row; a call of one workgroup without a mask needs none
 constexpr long long SINGLE = 4096;
 // Up to this many rows every workgroup adds their lengths up for itself, which saves a launch: 1024 x 1024 float32 with lengths
-// 12.7 us against 14.5, 2048 x 1024 16.3 and 17.2, 4096 x 1024 24.7 and 22.5, 16384 x 1024 71 and 53.
+// 12.5 us against 14.3, 2048 x 1024 16.4 and 17.2, 4096 x 1024 25.3 and 23.0, 16384 x 1024 76 and 58.
 constexpr long long COUNT_ROWS = 2048;
 size_t policy_bytes(const trebi_token_desc& d) {
   if (!d.mask && d.rows >= 0 && d.rows <= SINGLE && d.len >= 0 && (d.packed || d.len <= SINGLE) && (d.packed ? d.len : d.rows * d.len) <= SINGLE) return 0;
@@ -95,16 +95,16 @@ size_t policy_bytes(const trebi_token_desc& d) {
 
 constexpr int PAIR_BLOCKS = 2048;
 // Rows are split over workgroups where whole pairs would leave the card idle: at most one pair a CU, and rows long enough to
-// pay for the second read and the third launch.  float32: 24 pairs of 131072 tokens 22 us, whole 80; 24 x 16384 10 and 15; 100 x
-// 16384 17 both ways; 250 x 16384 25, whole 22; 24 x 8192 10 both ways.  (Lengths on the device do not matter for the choice.)
+// pay for the second read and the third launch.  float32: 24 pairs of 131072 tokens 23 us, whole 88; 24 x 16384 10 and 16; 100 x
+// 16384 17.5 and 19; 250 x 16384 27, whole 23; 24 x 8192 10 both ways.  (Lengths on the device do not matter for the choice.)
 int pair_splits(const trebi_token_desc& d) {
   const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len;
   if (d.rows > 512 || len <= 8192 || len < 64 * d.rows) return 0;
   return (int)std::max<long long>(1, std::min<long long>(PAIR_BLOCKS / d.rows, (len + 4095) / 4096));
 }
 // Threads of a pair.  A wave pays for its pairs' scalars (a few hundred instructions) whatever it holds: few pairs take a whole
-// workgroup each, many pairs of short rows 16 threads.  bfloat16, us with 16 / 64 / 256 threads: 512 pairs of 60 tokens 7.5 / 7.7 /
-// 7.7, of 500 10.7 / 8.0 / 7.6, of 2000 25 / 12 / 8.5; 2000 of 1000 17 / 12 / 15; 8000 of 200 11 / 17 / 33.
+// workgroup each, many pairs of short rows 16 threads.  bfloat16, us with 16 / 64 / 256 threads: 512 pairs of 60 tokens 7.7 / 8.2 /
+// 7.9, of 500 11 / 8.1 / 7.8, of 2000 27 / 12 / 9.5; 2000 of 1000 18 / 13 / 18; 8000 of 200 12 / 19 / 39.
 int pair_group(const trebi_token_desc& d) {
   const long long len = d.packed ? (d.len + d.rows - 1) / d.rows : d.len, pairs = d.rows / 2;
   if (len <= 128 || (pairs > 4096 && len <= 512)) return 16;
@@ -244,7 +244,7 @@ extern "C" int trebi_policy_loss(trebi_ctx* ctx, const trebi_token_desc* tokens,
   p.stats = d->stats;
   TokenP& t = p.tk;
   // Rows of one token are one row of tokens, to either mean, and that goes 16 bytes a thread instead of token by token (4 M
-  // float32: 20 us, as rows 31; bfloat16 17 and 35)
+  // float32: 20 us, as rows 31; bfloat16 18 and 35)
   if (!t.packed && t.len == 1 && !t.lengths && (!t.mask || t.mrs == 1)) {
     t.len = t.rows;
     t.rows = 1;

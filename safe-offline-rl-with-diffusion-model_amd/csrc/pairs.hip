@@ -1,8 +1,8 @@
 // Preference loss over paired log ratios, and its gradient.
 //
 // Bound by memory where rows are long: 250 pairs of 65536 float32 tokens, 393 MB, 89 us, 4.4 TB/s.  Few or short pairs are
-// bound by the launches and one pass of latency (16 pairs of 20 tokens 4.6 us, 512 packed pairs of 1023 9.7), many short ones by the
-// pairs' scalars (30000 pairs of 20: 17 us).  The gradient of a token is the same in its whole row, so it is written, not
+// bound by the launches and one pass of latency (16 pairs of 20 tokens 4.7 us, 512 packed pairs of 1023 10.4), many short ones by the
+// pairs' scalars (30000 pairs of 20: 18 us, of which the sigmoid in float64 costs 1.4).  The gradient of a token is the same in its whole row, so it is written, not
 // computed; the row has to be summed before.  Sums are taken in float64, in a fixed order, and a one-workgroup kernel adds the
 // workgroups' partial sums (2.5 us; no atomics: results do not change from run to run).
 #include "finetune.h"
@@ -168,7 +168,7 @@ __device__ __forceinline__ void pair_gaps(const PairP& p) {
 // G threads take a pair, half of them a row: the rows' sums, the pair, the rows' gradients.  Where there are pairs enough
 // to fill the card this is one pass: the gradient needs no second read of the log-probabilities.  A workgroup takes 256 / G
 // pairs and ends: in a loop over pairs the compiler kept what does not change in registers, 190 of them (8000 pairs of 200
-// float32 tokens, 64 threads each: 27 us, now 17).  Four waves a SIMD: with five the 16-bit kernels spill and gain nothing.
+// float32 tokens, 64 threads each: 27 us, now 19).  Four waves a SIMD: with five the 16-bit kernels spill and gain nothing.
 template <typename T, int G>
 __global__ __launch_bounds__(256, 4) void pairs_whole_kernel(PairP p) {
   __shared__ double lds[20];
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256, 4) void pairs_whole_kernel(PairP p) {
 }
 
 // Few pairs of long rows: `splits` workgroups sum a row, then as many write its gradient.  24 pairs of 131072 float32 tokens, 63 MB:
-// 9.7 us for the sums, 9.8 for the gradient (25 MB: bound by the latency of the parts it begins with).
+// 9.8 us for the sums, 9.3 for the gradient (25 MB: bound by the latency of the parts it begins with).
 __device__ __forceinline__ void split_of(long long s, long long e, int splits, int j, long long* a, long long* b) {
   const long long w = ((e - s + splits - 1) / splits + 511) / 512 * 512;         // whole waves of 8 tokens a lane
   *a = s + w * j < e ? s + w * j : e;

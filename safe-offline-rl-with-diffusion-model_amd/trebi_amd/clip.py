@@ -5,8 +5,10 @@
     flat, norm = clipper.clip_into(1.0, grad_scale=1 / loss_scale)   # float32 copies, back to back, gradients untouched
 
 With s = grad_scale:  n = s * ||all gradients||,  every gradient becomes s * min(1, max_norm / (n + 1e-6)) * g
-(torch.nn.utils.clip_grad_norm_'s arithmetic; the sum is taken in float64).  The norm comes back as a device tensor: no call
-here waits for the GPU.  training.Trainer(max_grad_norm=...) clips its flat gradient inside the optimiser step instead.
+(torch.nn.utils.clip_grad_norm_'s arithmetic; the sum is taken in float64).  The norm comes back as a device tensor: a
+GradClipper's calls do not wait for the GPU.  Making one does (its table is copied to the device), and so does the function
+clip_grad_norm_, which makes one in every call.  training.Trainer(max_grad_norm=...) clips its flat gradient inside the
+optimiser step instead.
 The reference trains without clipping.
 """
 import ctypes as C
@@ -28,8 +30,8 @@ def _norm_kind(norm_type):
 
 class GradClipper:
     """Bound to a list of CUDA gradients (float32, bfloat16 and float16 may be mixed; contiguous; none twice): holds them and
-    the device table of their places.  Make a new one when a gradient is allocated anew, and keep it as long as graphs that
-    captured its calls.  Making one copies the table to the device, so it cannot be captured; the calls can."""
+    the device table of their places.  Make a new one when a gradient is allocated anew (zero_grad(set_to_none=True), torch's
+    default, leaves .grad to be: this one would go on with the old tensors), and keep it as long as graphs that captured its calls.  Making one copies the table to the device, so it cannot be captured; the calls can."""
 
     def __init__(self, tensors, norm_type=2.0):
         self.tensors = list(tensors)
@@ -100,8 +102,8 @@ class GradClipper:
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """torch.nn.utils.clip_grad_norm_ for one call: clips the .grad of `parameters` in place and returns their norm.  A program
-    that clips every step keeps a GradClipper instead; error_if_nonfinite waits for the GPU."""
+    """torch.nn.utils.clip_grad_norm_ for one call: clips the .grad of `parameters` in place and returns their norm.  Waits for the
+    copy of the table, with error_if_nonfinite for the norm too; a program that clips every step keeps a GradClipper instead."""
     if torch.is_tensor(parameters):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]

@@ -180,7 +180,7 @@ def preference_loss(logp, logp_ref=None, *, mask=None, lengths=None, cu_seqlens=
 
         D_r = sum over the row's valid tokens of logp - logp_ref   (no logp_ref: logp; average: divided by their number)
         h = D_k - D_{k+P},  z = beta h - margin
-        'sigmoid': -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing
+        'sigmoid': -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing (which the other kinds do not have: no effect there)
         'hinge':   max(0, 1 - z)
         'ipo':     (z / beta - 1 / (2 beta))^2
         loss = sum_k weights[k] l_k / P     (denominator instead of P where given; data-parallel: the global number of pairs)
