@@ -1,8 +1,8 @@
 // Clipped policy loss with a KL term, and its gradient: the kernels, for one element type (policy_f32.hip and its likes).
 //
 // A token costs 2..4 loads, one store and some tens of instructions.  4.2 M packed float32 tokens, three inputs, an advantage a token,
-// a gradient: 83 MB, 25.6 us, 3.3 TB/s; the vector units issue half of the time.  4096 x 8192 padded bfloat16 tokens, of which 0.75 count,
-// second KL term: 218 MB, 60 us, 3.7 TB/s; 60 vector instructions for each 64 tokens that count, which the vector units issue in 64 % of
+// a gradient: 83 MB, 25.7 us, 3.2 TB/s; the vector units issue 42 % of the time.  4096 x 8192 padded bfloat16 tokens, of which 0.75 count,
+// second KL term: 218 MB, 60 us, 3.7 TB/s; 60 vector instructions for each 64 tokens that count, which the vector units issue in 61 % of
 // the time.  Inputs are read once and the gradient leaves in the same pass; scalars are summed in float64, in a fixed order, and a
 // one-workgroup kernel adds the workgroups' partial sums (4 us; no atomics: results do not change from run to run).
 #include "finetune.h"
